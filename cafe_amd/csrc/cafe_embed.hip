@@ -1532,7 +1532,7 @@ static int step_common(cafe_sketch_t *s, cafe_tables_t *t, const StepArgs &a, ca
                 if (backward_common(t, d_fields, d_que, d_grad_out, batch, total, lr, st, side, split ? 17 : 1, nullptr, 0, gstride)) return 1;
                 plan_done = true;
                 if (split) {
-                    // The gradient pass (segment sums; tables untouched) on the low-priority stream: behind the norm
+                    // The gradient pass (segment sums; tables untouched) on the third stream: behind the norm
                     // kernel (which read the same gradient: it is complete) and the partition passes.  It runs while the
                     // insert's latency-bound kernels leave the memory system idle; the row updates follow the migration.
                     CAFE_HIP_CHECK(hipStreamWaitEvent(s->low_stream, s->ev_gn, 0));

@@ -70,7 +70,7 @@ struct cafe_sketch {
     // partition offsets, item records) and the partition passes of the backward run there, beside the score kernel on
     // the caller's stream (cafe_backward_update_dev).
     hipStream_t side_stream = nullptr;
-    // Third stream, lowest priority: the gradient pass of the split update (segment sums) beside the insert's kernels
+    // Third stream: the gradient pass of the split update (segment sums) beside the insert's kernels
     hipStream_t low_stream = nullptr;
     hipEvent_t ev_gn = nullptr;         // completion of the norm kernel (it read the gradient: the gradient is ready)
     int opt_split_update = 1;
@@ -164,7 +164,7 @@ struct cafe_tables {
     // whose lookups mostly hit distinct rows gains nothing from the split (the sums travel through memory once more)
     uint32_t *h_rows = nullptr;
     int split_pause = 0;                // steps left before the split form is tried again
-    hipEvent_t ev_sums = nullptr;    // segment sums of the split update done (recorded on the sketch's low-priority stream)
+    hipEvent_t ev_sums = nullptr;    // segment sums of the split update done (recorded on the sketch's third stream)
 };
 
 namespace cafe {

@@ -354,17 +354,11 @@ static int run_reset(cafe_sketch *s, hipStream_t st) {
 // more queues than the hardware schedules at once).
 int cafe::ensure_streams(cafe_sketch *s) {
     if (s->side_stream) return 0;
-    // the second stream carries the short plan kernels beside the bandwidth kernels: highest priority, so that their
-    // workgroups are placed as soon as compute-unit slots free up
-    int prio_least = 0, prio_most = 0;
-    CAFE_HIP_CHECK(hipDeviceGetStreamPriorityRange(&prio_least, &prio_most));
-    CAFE_HIP_CHECK(hipStreamCreateWithPriority(&s->side_stream, hipStreamNonBlocking, prio_most));
-    // The third one carries a bandwidth kernel beside the insert's short kernels.  Default priority, not the lowest: the
-    // caller's stream waits for this one (the row updates wait for the segment sums), and in a process that holds more
-    // queues than the hardware schedules at once a lowest-priority queue was never scheduled while the waiting queue
-    // counted as busy (a full test session hung at the first step of its 29th test).
-    (void)prio_least;
-    CAFE_HIP_CHECK(hipStreamCreateWithPriority(&s->low_stream, hipStreamNonBlocking, 0));
+    // The second stream carries the short plan kernels beside the bandwidth kernels, the third a bandwidth kernel beside
+    // the insert's short kernels.  Both at the default priority: streams of different priorities in one process have
+    // left a queue that another one waited for unscheduled.
+    CAFE_HIP_CHECK(hipStreamCreateWithFlags(&s->side_stream, hipStreamNonBlocking));
+    CAFE_HIP_CHECK(hipStreamCreateWithFlags(&s->low_stream, hipStreamNonBlocking));
     return 0;
 }
 
