@@ -12,6 +12,7 @@ _u32p = ctypes.POINTER(ctypes.c_uint32)
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 _f32p = ctypes.POINTER(ctypes.c_float)
 _vp = ctypes.c_void_p
+_i64 = ctypes.c_int64
 
 # every symbol include/cafe_hip.h declares: (restype, argtypes)
 SYMBOLS = {
@@ -85,6 +86,12 @@ SYMBOLS = {
     "cafe_route_ws_words": (ctypes.c_int, [ctypes.c_int, ctypes.c_int]),
     "cafe_route_dev": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp]),
     "cafe_split_ids_dev": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
+    "cafe_linear_fwd_ws": (_i64, [_i64, _i64, _i64, ctypes.c_int]),
+    "cafe_linear_fwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
+                                           ctypes.c_int, ctypes.c_int, _vp, _i64, _vp]),
+    "cafe_linear_bwd_ws": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
+    "cafe_linear_bwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
+                                           ctypes.c_int, ctypes.c_int, _vp, _i64, _vp]),
     "cafe_grad_norm_dev": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]),
 }
 
