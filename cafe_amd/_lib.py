@@ -92,6 +92,12 @@ SYMBOLS = {
     "cafe_linear_bwd_ws": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "cafe_linear_bwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
                                            ctypes.c_int, ctypes.c_int, _vp, _i64, _vp]),
+    "cafe_interact_fwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i64] + [ctypes.c_int] * 5 + [_vp, _i64, _vp]),
+    "cafe_interact_bwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64] + [ctypes.c_int] * 5
+                              + [_vp, _i64, _vp, _i64, _i64, _vp]),
+    "cafe_adamw_dev": (ctypes.c_int, [_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
+    "cafe_adamw_tick_dev": (ctypes.c_int, [_vp, _vp] + [ctypes.c_double] * 4 + [_vp, _vp]),
+    "cafe_moment8_values_dev": (ctypes.c_int, [_i64p, ctypes.c_int, _vp]),
     "cafe_grad_norm_dev": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]),
 }
 

@@ -1,0 +1,261 @@
+"""AdamW over many tensors in one launch (cafe_amd/csrc/cafe_adamw.hip), moments in 32 or 8 bits.
+
+The dense parameters of a head are a dozen tensors between one value and a few million; the reference steps them with
+torch.optim.  `AdamW` is a torch.optim.Optimizer; `adamw_step` the step itself over lists
+of tensors; `moment8_values` the float32 values that 8-bit moments stand for."""
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .linear import DTYPE_CODE, launch_on, on_device
+
+BLOCK = 256                     # values that share one exponent
+
+
+class Moment8(NamedTuple):
+    """A moment in 8 bits: a code per value of the flattened tensor and an exponent (plus 127) per 256 of them."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+
+    @classmethod
+    def zeros(cls, n, device):
+        return cls(torch.zeros(n, dtype=torch.uint8, device=device),
+                   torch.ones(-(-n // BLOCK), dtype=torch.uint8, device=device))
+
+
+def _check_moment8(m, n, device, what):
+    if not isinstance(m, Moment8):
+        raise ValueError(f"{what}: Moment8 expected beside Moment8, not {type(m).__name__}")
+    c, e = m
+    if (c.dtype is not torch.uint8 or e.dtype is not torch.uint8 or c.numel() != n or e.numel() != -(-n // BLOCK)
+            or c.device != device or e.device != device or not c.is_contiguous() or not e.is_contiguous()):
+        raise ValueError(f"{what}: {n} uint8 codes and {-(-n // BLOCK)} uint8 exponents, contiguous, on {device} expected")
+
+
+def _check_float(t, shape, device, what):
+    if t.dtype is not torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous float32 {tuple(shape)} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+               masters=None, factors=None):
+    """One AdamW step in place over lists of tensors:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+
+    params: contiguous, of one type (float32, bfloat16, float16), on one GPU, no two sharing memory; grads: of the same
+    type and shape.  exp_avgs, exp_avg_sqs: float32 tensors of the parameter's shape, or Moment8 throughout.  masters:
+    None, or float32 tensors of the parameters' shapes that are updated in their place; the parameters then receive the
+    rounded values.  step: the number of this step, from 1; it is a number of the host, so a call under graph capture
+    takes `factors` instead (adamw_tick), a float32 tensor of three on the device.  All arithmetic is float32."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or (masters is not None and len(masters) != n):
+        raise ValueError("params, grads, moments and masters are lists of one length")
+    if n == 0:
+        return
+    first = params[0]
+    dtype, device = first.dtype, first.device
+    if dtype not in DTYPE_CODE:
+        raise ValueError(f"float32, bfloat16 or float16 parameters expected, not {dtype}")
+    eight = isinstance(exp_avgs[0], Moment8)
+    cols = [[], [], [], [], [0] * n, [0] * n, [0] * n, []]
+    if eight:
+        cols[4], cols[5] = [], []
+    held = []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if p.dtype is not dtype or p.device != device or not p.is_contiguous():
+            raise ValueError(f"params[{i}]: contiguous {dtype} on {device} expected, got {p.dtype} on {p.device}")
+        if g.dtype is not dtype or g.shape != p.shape or g.device != device or g.layout is not torch.strided:
+            raise ValueError(f"grads[{i}]: dense {dtype} {tuple(p.shape)} on {device} expected, got {g.dtype} {tuple(g.shape)} on {g.device}")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            held.append(g)
+        count = p.numel()
+        if eight:
+            _check_moment8(m, count, device, f"exp_avgs[{i}]")
+            _check_moment8(v, count, device, f"exp_avg_sqs[{i}]")
+            cols[2].append(m.codes.data_ptr())
+            cols[3].append(v.codes.data_ptr())
+            cols[4].append(m.exponents.data_ptr())
+            cols[5].append(v.exponents.data_ptr())
+        else:
+            if isinstance(m, Moment8) or isinstance(v, Moment8):
+                raise ValueError(f"moments of tensor {i}: float32 tensors expected beside float32 tensors")
+            _check_float(m, p.shape, device, f"exp_avgs[{i}]")
+            _check_float(v, p.shape, device, f"exp_avg_sqs[{i}]")
+            cols[2].append(m.data_ptr())
+            cols[3].append(v.data_ptr())
+        cols[0].append(p.data_ptr())
+        cols[1].append(g.data_ptr())
+        cols[7].append(count)
+    if masters is not None:
+        for i, (p, w) in enumerate(zip(params, masters)):
+            _check_float(w, p.shape, device, f"masters[{i}]")
+        cols[6] = [w.data_ptr() for w in masters]
+    used = [a for a, c in zip(cols[0], cols[7]) if c]
+    if len(set(used)) != len(used):
+        raise ValueError("a parameter is listed twice")
+    on_device(first)
+    if factors is None:
+        if step is None or int(step) != step or step < 1:
+            raise ValueError(f"step {step}: the number of this step, from 1, or `factors`")
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.CafeError("a captured step would repeat the same step number: use adamw_tick and `factors`")
+        step = int(step)
+    else:
+        _check_float(factors, torch.Size((3,)), device, "factors")
+        step = 0
+    flat = (ctypes.c_int64 * (8 * n))(*[a for c in cols for a in c])
+    with launch_on(first) as st:
+        _lib.check(_lib.load().cafe_adamw_dev(flat, n, DTYPE_CODE[dtype], 8 if eight else 32, float(lr), float(betas[0]), float(betas[1]),
+                                              float(eps), float(weight_decay), step, None if factors is None else factors.data_ptr(), st),
+                   "cafe_adamw_dev")
+
+
+def adamw_tick(step, factors, *, lr, betas=(0.9, 0.999), weight_decay=0.01):
+    """step (an int64 tensor of one on the device) += 1, and `factors` (float32, three) for that step of adamw_step.  lr: a
+    number, or a float32 tensor of one on the same device that is read when the launch runs.  May be captured."""
+    if step.dtype is not torch.int64 or step.numel() != 1 or factors.device != step.device:
+        raise ValueError("step: an int64 tensor of one element, on the device of `factors`")
+    _check_float(factors, torch.Size((3,)), step.device, "factors")
+    ptr = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != step.device:
+            raise ValueError("lr: a number or a float32 tensor of one element on the device of `step`")
+        ptr, lr = lr.data_ptr(), 0.0
+    on_device(step)
+    with launch_on(step) as st:
+        _lib.check(_lib.load().cafe_adamw_tick_dev(step.data_ptr(), ptr, float(lr), float(betas[0]), float(betas[1]),
+                                                   float(weight_decay), factors.data_ptr(), st), "cafe_adamw_tick_dev")
+
+
+def moment8_values(exp_avgs, exp_avg_sqs):
+    """The float32 values (1-d tensors) that two lists of Moment8 stand for, first moments and second moments, in one launch."""
+    both = [(m, 0) for m in exp_avgs] + [(v, 1) for v in exp_avg_sqs]
+    if not both:
+        return [], []
+    device = both[0][0].codes.device
+    cols, out = [[], [], [], [], []], []
+    for m, second in both:
+        n = m.codes.numel()
+        _check_moment8(m, n, device, "moment")
+        out.append(torch.empty(n, dtype=torch.float32, device=device))
+        for c, a in zip(cols, (m.codes.data_ptr(), m.exponents.data_ptr(), out[-1].data_ptr(), n, second)):
+            c.append(a)
+    on_device(both[0][0].codes)
+    flat = (ctypes.c_int64 * (5 * len(both)))(*[a for c in cols for a in c])
+    with launch_on(both[0][0].codes) as st:
+        _lib.check(_lib.load().cafe_moment8_values_dev(flat, len(both), st), "cafe_moment8_values_dev")
+    return out[:len(exp_avgs)], out[len(exp_avgs):]
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update in one launch per type and step count.
+
+    state_bits: 32, or 8 for moments of one byte per value (plus one per 256).  master_weights: bfloat16 and float16
+    parameters keep a float32 copy that the steps accumulate in (default True; ignored for float32).  capturable: the
+    step count of a parameter group lives on the device, so that step() can be captured into a graph and replayed; lr may
+    then be a float32 tensor of one element on the device, and parameters without a gradient are skipped but do not lag
+    behind the group's count.  Parameters are contiguous; sparse gradients are refused."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, master_weights=True,
+                 capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits {state_bits}: 8 or 32")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("lr as a tensor needs capturable=True")
+        for name, v, ok in (("lr", lr, isinstance(lr, torch.Tensor) or lr >= 0), ("eps", eps, eps >= 0),
+                            ("weight_decay", weight_decay, weight_decay >= 0),
+                            ("betas", betas, all(0 <= b < 1 for b in betas) and len(betas) == 2)):
+            if not ok:
+                raise ValueError(f"{name} {v}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, capturable=capturable))
+
+    def _init_state(self, p, group):
+        st = self.state[p]
+        st["step"] = 0
+        if group["state_bits"] == 8:
+            for name in ("exp_avg", "exp_avg_sq"):
+                st[name + "_codes"], st[name + "_exponents"] = Moment8.zeros(p.numel(), p.device)
+        else:
+            st["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype is not torch.float32:
+            st["master"] = p.detach().float().clone(memory_format=torch.contiguous_format)
+        return st
+
+    @staticmethod
+    def _moments(st):
+        if "exp_avg_codes" in st:
+            return Moment8(st["exp_avg_codes"], st["exp_avg_exponents"]), Moment8(st["exp_avg_sq_codes"], st["exp_avg_sq_exponents"])
+        return st["exp_avg"], st["exp_avg_sq"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            sets = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.layout is not torch.strided:
+                    raise ValueError("sparse gradients are not supported: the sketch-backed tables have their own update")
+                st = self.state[p] if self.state.get(p) else self._init_state(p, group)
+                if not group["capturable"]:
+                    st["step"] += 1
+                key = (p.device, p.dtype, st["step"], "exp_avg_codes" in st, "master" in st)
+                sets.setdefault(key, []).append((p, st))
+            ticked = {}
+            for (device, _, step, _, master), members in sets.items():
+                kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step)
+                if group["capturable"]:
+                    if device not in ticked:
+                        ticked[device] = self._tick(group, device)
+                    kw.update(step=None, lr=0.0, factors=ticked[device])
+                moments = [self._moments(st) for _, st in members]
+                adamw_step([p for p, _ in members], [p.grad for p, _ in members], [m for m, _ in moments], [v for _, v in moments],
+                           masters=[st["master"] for _, st in members] if master else None, **kw)
+        return loss
+
+    @staticmethod
+    def _tick(group, device):
+        """The group's device-side count on `device`, advanced, and its factors."""
+        counts = group.setdefault("device_step", {})
+        key = str(device)
+        if key not in counts:
+            if torch.cuda.is_current_stream_capturing():
+                raise _lib.CafeError("run one step before the capture: it creates the device-side step count")
+            counts[key] = (torch.zeros(1, dtype=torch.int64, device=device), torch.empty(3, dtype=torch.float32, device=device))
+        count, factors = counts[key]
+        adamw_tick(count, factors, lr=group["lr"], betas=group["betas"], weight_decay=group["weight_decay"])
+        return factors
+
+    def state_dict(self):
+        out = super().state_dict()
+        for group in out["param_groups"]:
+            if "device_step" in group:
+                group["device_step"] = {k: int(c) for k, (c, _) in group["device_step"].items()}
+        return out
+
+    def load_state_dict(self, state_dict):
+        """torch's, except that moments, codes and master weights keep their own types (torch casts floating state to the
+        parameter's)."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, mine):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.detach().to(p.device).clone() if isinstance(v, torch.Tensor) else v
+                                 for k, v in state_dict["state"][i].items()}
+        for group in self.param_groups:
+            counts = group.pop("device_step", None)
+            if counts:
+                group["device_step"] = {k: (torch.full((1,), int(c), dtype=torch.int64, device=k),
+                                            torch.empty(3, dtype=torch.float32, device=k)) for k, c in counts.items()}

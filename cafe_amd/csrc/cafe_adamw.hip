@@ -1,0 +1,316 @@
+// cafe_adamw.hip -- one AdamW step over many tensors in one launch, moments in float32 or in 8 bits:
+//
+//     m = b1 m + (1 - b1) g     v = b2 v + (1 - b2) g^2
+//     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// for the dense parameters of the models' heads (the reference steps them
+// with torch.optim).  All arithmetic is float32, operation by operation as written (no contraction), so the
+// 8-bit codes do not depend on how a compiler fuses.  Bound by memory: 28 bytes per float32 value with float32 moments,
+// 16 with 8-bit ones.
+//
+// 8-bit moments.  256 consecutive values share an exponent E, that of the largest finite magnitude among them (at least
+// -126; stored plus 127).  A value is scaled by 2^-E -- exactly -- into [0, 2) and rounded to nearest even in a small
+// floating format: m has a sign, 4 exponent and 3 mantissa bits (0x80: not finite, read as NaN), v 5 and 3 (0xff: not
+// finite, read as infinity).  Half a step is 2^-4 of a value over 14 and 30 binades.  The update uses the fresh float32
+// m and v; only what the next step reads is rounded.  A v above 0 is never stored as 0: next step's division by
+// sqrt(v) would blow its m up.  (v loses accuracy only where it is 2^-30 of its block's largest.)
+#include "cafe_dense.h"
+
+#include <algorithm>
+#include <math.h>
+
+using namespace cafe;
+
+namespace {
+
+constexpr int kItems = 48;              // tensors of one launch: their descriptors travel as kernel arguments (4 KB at most)
+constexpr int kSpan = 4096;             // values per workgroup: 4 waves x 4 blocks of 256
+constexpr int kBlock = 256;
+
+struct Item { void *p; const void *g; void *m, *v; uint8_t *me, *ve; float *w; int64_t n; };
+struct AdamArgs {
+    Item t[kItems];
+    int32_t first[kItems + 1];          // first workgroup of every tensor
+    const float *factors;               // device: {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd}, or null
+    float step_size, root, keep, b1, c1, b2, c2, eps;
+    int count;
+};
+static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
+
+template <class T> struct Four;         // four elements, at element alignment
+template <> struct Four<float> { struct __attribute__((packed, aligned(4))) V { u32x4 v; }; };
+template <> struct Four<__bf16> { struct __attribute__((packed, aligned(2))) V { u32x2 v; }; };
+template <> struct Four<_Float16> { struct __attribute__((packed, aligned(2))) V { u32x2 v; }; };
+template <> struct Four<uint8_t> { struct __attribute__((packed, aligned(1))) V { uint32_t v; }; };
+
+template <class T, class F> __device__ __forceinline__ void get4(const T *p, int n, F *out) {
+    union { typename Four<T>::V v; T e[4]; } u;
+    if (n >= 4) {
+        u.v = *(const typename Four<T>::V *)p;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = (F)u.e[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = i < n ? (F)p[i] : (F)0;
+    }
+}
+template <class T, class F> __device__ __forceinline__ void put4(T *p, int n, const F *in) {
+    union { typename Four<T>::V v; T e[4]; } u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) u.e[i] = (T)in[i];
+    if (n >= 4) *(typename Four<T>::V *)p = u.v;
+    else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < n) p[i] = u.e[i];
+    }
+}
+
+// exponent of |x| with that of 0 and of subnormals taken as -127 (callers clamp)
+__device__ __forceinline__ int exponent_of(float mag) { return (int)(__float_as_uint(mag) >> 23) - 127; }
+
+template <bool SECOND> __device__ __forceinline__ float decode8(int c, int e) {
+    constexpr int low = SECOND ? -30 : -14;
+    const int mag = SECOND ? c : c & 0x7f, field = mag >> 3;
+    const float v = ldexpf((float)(field ? 8 + (mag & 7) : mag & 7), (field ? field - 1 : 0) + low - 3 + e);
+    if (SECOND) return c == 0xff ? INFINITY : v;
+    return c == 0x80 ? NAN : c & 0x80 ? -v : v;
+}
+template <bool SECOND> __device__ __forceinline__ int encode8(float x, int e) {
+    constexpr int low = SECOND ? -30 : -14;
+    const float mag = fabsf(x);
+    if (!(mag <= 3.4028234663852886e38f)) return SECOND ? 0xff : 0x80;
+    const float a = ldexpf(mag, -e);
+    const int b = max(exponent_of(a), low);
+    int c = (int)rintf(ldexpf(a, 3 - b)) + 8 * (b - low);
+    if (SECOND) {
+        c = min(c, 0xfe);
+        return c == 0 && mag > 0.f ? 1 : c;
+    }
+    c = min(c, 0x7f);
+    return x < 0.f && c > 0 ? c | 0x80 : c;
+}
+// exponent of a block of 256 values, four per lane of one wave
+__device__ __forceinline__ int block_exponent(const float *x) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float mag = fabsf(x[i]);
+        if (mag <= 3.4028234663852886e38f) top = fmaxf(top, mag);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    return max(exponent_of(top), -126);
+}
+
+__device__ __forceinline__ int item_of(const int32_t *first, int count, int block) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= block) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
+    const int k = item_of(a.first, a.count, blockIdx.x);
+    const Item t = a.t[k];
+    float step_size = a.step_size, root = a.root, keep = a.keep;
+    if (a.factors) { step_size = a.factors[0]; root = a.factors[1]; keep = a.factors[2]; }
+    const int64_t base = (int64_t)(blockIdx.x - a.first[k]) * kSpan;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int u = 0; u < kSpan / kBlock / 4; u++) {
+        const int64_t block = base / kBlock + u * 4 + wave, at = block * kBlock + lane * 4;
+        if (block * kBlock >= t.n) return;
+        const int n = (int)(t.n - at < 4 ? t.n - at : 4);              // may be <= 0
+        float p[4], g[4], m[4], v[4];
+        get4((const T *)t.g + at, n, g);
+        if (t.w) get4(t.w + at, n, p);
+        else get4((const T *)t.p + at, n, p);
+        if (BITS8) {
+            int cm[4], cv[4];
+            get4((const uint8_t *)t.m + at, n, cm);
+            get4((const uint8_t *)t.v + at, n, cv);
+            const int em = (int)t.me[block] - 127, ev = (int)t.ve[block] - 127;
+#pragma unroll
+            for (int i = 0; i < 4; i++) { m[i] = decode8<false>(cm[i], em); v[i] = decode8<true>(cv[i], ev); }
+        } else {
+            get4((const float *)t.m + at, n, m);
+            get4((const float *)t.v + at, n, v);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            m[i] = m[i] * a.b1 + g[i] * a.c1;
+            v[i] = v[i] * a.b2 + (g[i] * g[i]) * a.c2;
+            const float denom = sqrtf(v[i]) * root + a.eps;
+            p[i] = p[i] * keep - (m[i] / denom) * step_size;
+        }
+        if (BITS8) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i >= n) m[i] = v[i] = 0.f;
+            const int em = block_exponent(m), ev = block_exponent(v);
+            int cm[4], cv[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { cm[i] = encode8<false>(m[i], em); cv[i] = encode8<true>(v[i], ev); }
+            put4((uint8_t *)t.m + at, n, cm);
+            put4((uint8_t *)t.v + at, n, cv);
+            if (lane == 0) { t.me[block] = (uint8_t)(em + 127); t.ve[block] = (uint8_t)(ev + 127); }
+        } else {
+            put4((float *)t.m + at, n, m);
+            put4((float *)t.v + at, n, v);
+        }
+        if (t.w) put4(t.w + at, n, p);
+        put4((T *)t.p + at, n, p);
+    }
+}
+
+struct ValueItem { const uint8_t *codes, *exps; float *out; int64_t n; };
+struct ValueArgs {
+    ValueItem t[2 * kItems];
+    int32_t first[2 * kItems + 1];
+    uint8_t second[2 * kItems];
+    int count;
+};
+static_assert(sizeof(ValueArgs) <= 4096, "kernel arguments");
+
+__global__ __launch_bounds__(256) void k_moment_values(ValueArgs a) {
+    const int k = item_of(a.first, a.count, blockIdx.x);
+    const ValueItem t = a.t[k];
+    const bool second = a.second[k];
+    const int64_t base = (int64_t)(blockIdx.x - a.first[k]) * kSpan;
+    for (int u = 0; u < kSpan / 1024; u++) {
+        const int64_t at = base + u * 1024 + threadIdx.x * 4;
+        if (at >= t.n) return;
+        const int n = (int)(t.n - at < 4 ? t.n - at : 4), e = (int)t.exps[at / kBlock] - 127;
+        int c[4];
+        float v[4];
+        get4(t.codes + at, n, c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = second ? decode8<true>(c[i], e) : decode8<false>(c[i], e);
+        put4(t.out + at, n, v);
+    }
+}
+
+__global__ void k_adamw_tick(int64_t *step, const float *lr_dev, double lr, double b1, double b2, double wd, float *factors) {
+    const int64_t t = *step + 1;
+    *step = t;
+    if (lr_dev) lr = (double)*lr_dev;
+    factors[0] = (float)(lr / (1.0 - pow(b1, (double)t)));
+    factors[1] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    factors[2] = (float)(1.0 - lr * wd);
+}
+
+bool bad_hyper(const char *who, double lr, double b1, double b2, double eps, double wd) {
+    if (!(lr >= 0) || !(b1 >= 0 && b1 < 1) || !(b2 >= 0 && b2 < 1) || !(eps >= 0) || !(wd >= 0)) {
+        set_error("%s: lr, eps and weight decay must not be negative, betas lie in [0, 1)", who);
+        return true;
+    }
+    return false;
+}
+
+template <class T, bool BITS8> int launch(const AdamArgs &a, unsigned blocks, hipStream_t st) {
+    hipLaunchKernelGGL((k_adamw<T, BITS8>), dim3(blocks), dim3(256), 0, st, a);
+    CAFE_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
+                              double eps, double weight_decay, int64_t step, const float *d_factors, cafe_stream_t stream) {
+    if (count < 0 || (count && !tensors)) { set_error("cafe_adamw_dev: no tensor table"); return 1; }
+    if (dtype < kF32 || dtype > kF16 || (state_bits != 8 && state_bits != 32)) {
+        set_error("cafe_adamw_dev: type code %d, %d-bit states", dtype, state_bits);
+        return 1;
+    }
+    if (bad_hyper("cafe_adamw_dev", lr, beta1, beta2, eps, weight_decay)) return 1;
+    if (!d_factors && step < 1) { set_error("cafe_adamw_dev: step %lld, the first is 1", (long long)step); return 1; }
+    for (int i = 0; i < count; i++) {
+        const int64_t *c = tensors + i;
+        const int64_t n = c[7 * (int64_t)count];
+        bool null = false;
+        for (int f = 0; f < 4; f++) null |= c[f * (int64_t)count] == 0;
+        if (state_bits == 8) null |= c[4 * (int64_t)count] == 0 || c[5 * (int64_t)count] == 0;
+        if (n < 0 || n > ((int64_t)1 << 42) || (n > 0 && null)) {
+            set_error("cafe_adamw_dev: tensor %d has %lld values or a null pointer", i, (long long)n);
+            return 1;
+        }
+    }
+    AdamArgs a = {};
+    a.factors = d_factors;
+    if (!d_factors) {
+        a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+        a.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+        a.keep = (float)(1.0 - lr * weight_decay);
+    }
+    a.b1 = (float)beta1; a.c1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.c2 = (float)(1.0 - beta2); a.eps = (float)eps;
+    const hipStream_t st = (hipStream_t)stream;
+    int i = 0;
+    while (i < count) {
+        int64_t blocks = 0;
+        a.count = 0;
+        for (; i < count && a.count < kItems; i++) {
+            const int64_t n = tensors[7 * (int64_t)count + i], more = (n + kSpan - 1) / kSpan;
+            if (n == 0) continue;
+            if (a.count && blocks + more > INT32_MAX) break;
+            auto at = [&](int f) { return (void *)(uintptr_t)tensors[f * (int64_t)count + i]; };
+            a.t[a.count] = Item{at(0), at(1), at(2), at(3), (uint8_t *)at(4), (uint8_t *)at(5), (float *)at(6), n};
+            a.first[a.count++] = (int32_t)blocks;
+            blocks += more;
+        }
+        if (!a.count) break;
+        a.first[a.count] = (int32_t)blocks;
+        const unsigned b = (unsigned)blocks;
+        const bool s8 = state_bits == 8;
+        int rc;
+        if (dtype == kF32) rc = s8 ? launch<float, true>(a, b, st) : launch<float, false>(a, b, st);
+        else if (dtype == kBF16) rc = s8 ? launch<__bf16, true>(a, b, st) : launch<__bf16, false>(a, b, st);
+        else rc = s8 ? launch<_Float16, true>(a, b, st) : launch<_Float16, false>(a, b, st);
+        if (rc) return rc;
+    }
+    return 0;
+}
+
+extern "C" int cafe_adamw_tick_dev(int64_t *d_step, const float *d_lr, double lr, double beta1, double beta2, double weight_decay,
+                                   float *d_factors, cafe_stream_t stream) {
+    if (!d_step || !d_factors) { set_error("cafe_adamw_tick_dev: null pointer"); return 1; }
+    if (bad_hyper("cafe_adamw_tick_dev", lr, beta1, beta2, 0, weight_decay)) return 1;
+    hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(1), 0, (hipStream_t)stream, d_step, d_lr, lr, beta1, beta2, weight_decay, d_factors);
+    CAFE_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+extern "C" int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_stream_t stream) {
+    if (count < 0 || (count && !tensors)) { set_error("cafe_moment8_values_dev: no tensor table"); return 1; }
+    for (int i = 0; i < count; i++) {
+        const int64_t n = tensors[3 * (int64_t)count + i];
+        bool null = false;
+        for (int f = 0; f < 3; f++) null |= tensors[f * (int64_t)count + i] == 0;
+        if (n < 0 || n > ((int64_t)1 << 42) || (n > 0 && null)) {
+            set_error("cafe_moment8_values_dev: tensor %d has %lld values or a null pointer", i, (long long)n);
+            return 1;
+        }
+    }
+    ValueArgs a = {};
+    int i = 0;
+    while (i < count) {
+        int64_t blocks = 0;
+        a.count = 0;
+        for (; i < count && a.count < 2 * kItems; i++) {
+            auto at = [&](int f) { return tensors[f * (int64_t)count + i]; };
+            const int64_t n = at(3), more = (n + kSpan - 1) / kSpan;
+            if (n == 0) continue;
+            if (a.count && blocks + more > INT32_MAX) break;
+            a.t[a.count] = ValueItem{(const uint8_t *)(uintptr_t)at(0), (const uint8_t *)(uintptr_t)at(1), (float *)(uintptr_t)at(2), n};
+            a.second[a.count] = at(4) != 0;
+            a.first[a.count++] = (int32_t)blocks;
+            blocks += more;
+        }
+        if (!a.count) break;
+        a.first[a.count] = (int32_t)blocks;
+        hipLaunchKernelGGL(k_moment_values, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+        CAFE_HIP_CHECK(hipGetLastError());
+    }
+    return 0;
+}

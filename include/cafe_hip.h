@@ -346,6 +346,36 @@ int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d_x, int64_t
                         const void *d_kept, int64_t ldk, void *d_dx, int64_t lddx, void *d_dw, void *d_db, int64_t m, int64_t k,
                         int64_t n, int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream);
 
+/* DLRM's dot interaction (dlrm_s_pytorch.py:779-809).  Feature rows of sample b: t_0 = d_x[b] if d_x is not null, then one
+ * row per field, d_emb[f * field_stride + b * batch_stride ..+ dim].  out[b] = [d_x[b] | <t_i, t_j>: i ascending, j < i
+ * (j <= i with itself != 0)], ldo >= dim (with d_x) + pairs.  d_x and d_out are of type `dtype`; emb_dtype is float32 or
+ * the same.  Products and sums in float32.  At most 128 feature rows. */
+int cafe_interact_fwd_dev(const void *d_x, int64_t ldx, const void *d_emb, int64_t field_stride, int64_t batch_stride,
+                          int64_t batch, int fields, int dim, int itself, int emb_dtype, int dtype, void *d_out, int64_t ldo,
+                          cafe_stream_t stream);
+/* Its gradients: d_dx [B, dim] (null: not wanted, or no d_x), d_demb (null: not wanted; emb_dtype, own strides). */
+int cafe_interact_bwd_dev(const void *d_dout, int64_t lddo, const void *d_x, int64_t ldx, const void *d_emb,
+                          int64_t field_stride, int64_t batch_stride, int64_t batch, int fields, int dim, int itself,
+                          int emb_dtype, int dtype, void *d_dx, int64_t lddx, void *d_demb, int64_t dfield_stride,
+                          int64_t dbatch_stride, cafe_stream_t stream);
+
+/* One AdamW step in place over `count` tensors (the dense parameters of a head; the reference steps them with torch.optim).  `tensors` is a
+ * HOST array of eight columns of `count` int64 each, copied before the call returns: addresses of p, g, m, v, exponents of
+ * m, exponents of v (0 with 32-bit states), float32 master weights (0: none), number of values.  p and g are of type
+ * `dtype`, any element alignment; m and v float32 (state_bits 32) or one code per value with one exponent byte per 256
+ * values (state_bits 8; the format stands in cafe_adamw.hip).  No two tensors may overlap.
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * d_factors != null: {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd} are read from the device (cafe_adamw_tick_dev) and
+ * lr and step are not used, so that the call can be captured and replayed. */
+int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, int64_t step, const float *d_factors, cafe_stream_t stream);
+/* *d_step += 1, then d_factors[3] for that step.  d_lr != null: the learning rate is read from there. */
+int cafe_adamw_tick_dev(int64_t *d_step, const float *d_lr, double lr, double beta1, double beta2, double weight_decay,
+                        float *d_factors, cafe_stream_t stream);
+/* The float32 values that 8-bit moments stand for.  `tensors`: five columns of `count` int64: codes, exponents, float32
+ * output, number of values, 1 for a second moment. */
+int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
