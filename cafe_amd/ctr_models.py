@@ -1,8 +1,11 @@
 """Thin DLRM / WDL / DCN models on the CAFE embedding layer.
 
-Only what is needed to report losses on the hot path's configurations: the heads are stock torch ops on the GPU
-(they are not on the path this package accelerates); the embedding layer is cafe_amd.CafeEmbeddingCollection, i.e.
-the fused HIP launches.  Structure and initialisation follow the reference:
+The embedding layer is cafe_amd.CafeEmbeddingCollection, i.e. the fused HIP launches; the heads are stock torch ops by
+default (dense_ops="torch") or, with dense_ops="hip", the package's own launches over the same parameters: every layer
+with its bias and activation (and WDL's wide logit) through cafe_amd.linear, the interaction through cafe_amd.interact.
+dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; embedding rows and
+the loss stay float32; cafe_amd.adamw.AdamW keeps float32 master weights for such parameters).  Structure and
+initialisation follow the reference:
 
 * DLRM: bottom MLP -> dot interaction of [x] + embeddings, strictly-lower-triangle terms, concatenated behind x ->
   top MLP whose last layer is a sigmoid (dlrm_s_pytorch.py:213-251 create_mlp, :779-820 interact_features,
@@ -25,13 +28,16 @@ the fused HIP launches.  Structure and initialisation follow the reference:
 
 Call order of a training step is the reference's (dlrm_s_pytorch.py:1640-1658): forward, loss.backward(),
 insert_grad (scores -> sketch insert -> migration), optimizer step; the embedding tables' SGD runs inside the fused
-backward (CafeEmbeddingCollection.backward_update), the dense parameters use torch.optim.SGD."""
+backward (CafeEmbeddingCollection.backward_update), the dense parameters use torch.optim.SGD (or any optimizer:
+cafe_amd.adamw.AdamW steps them in one launch)."""
 import numpy as np
 import torch
 import torch.nn as nn
 
 from . import config as cfg
 from .collection import CafeEmbeddingCollection
+from .interact import dot_interaction
+from .linear import DTYPE_CODE, linear, run_mlp
 
 
 def create_mlp(ln, sigmoid_layer=-1, rng=None):
@@ -70,14 +76,19 @@ def interact_dot(x, ly, itself=False):
 
 
 class CafeCTRHead(nn.Module):
-    """Everything behind the embedding layer: pure torch, device-agnostic (the parity tests run a copy on the CPU
-    behind the oracle's embedding layer)."""
+    """Everything behind the embedding layer.  dense_ops="torch": pure torch, device-agnostic (the parity tests run a copy
+    on the CPU behind the oracle's embedding layer); "hip": the same parameters through the package's own launches."""
 
     def __init__(self, kind, num_fields, dim, dense_dim=13, ln_bot=None, ln_top=None, seed=123, train_cross=False,
-                 interaction_itself=False):
+                 interaction_itself=False, dense_ops="torch", dense_dtype=torch.float32):
         super().__init__()
         if kind not in ("dlrm", "wdl", "dcn"):
             raise ValueError(kind)
+        if dense_ops not in ("torch", "hip"):
+            raise ValueError(f"dense_ops {dense_ops!r}: 'torch' or 'hip'")
+        if dense_dtype not in DTYPE_CODE or (dense_ops == "torch" and dense_dtype != torch.float32):
+            raise ValueError(f"dense_dtype {dense_dtype}: float32, or bfloat16 / float16 with dense_ops='hip'")
+        self.dense_ops, self.dense_dtype = dense_ops, dense_dtype
         self.kind, self.dim, self.dense_dim, self.F = kind, int(dim), int(dense_dim), int(num_fields)
         self.interaction_itself = interaction_itself
         self.train_cross = train_cross
@@ -114,9 +125,30 @@ class CafeCTRHead(nn.Module):
                     self.register_buffer(f"cross_bias_{i}", b)
             self.last_layer = nn.Linear(in_dim + 256, 1)
             self.top_l = create_mlp(ln_top, len(ln_top) - 2, rng)
+        if dense_dtype != torch.float32:
+            self.to(dense_dtype)
+
+    def _forward_hip(self, dense, emb):
+        """forward() over cafe_amd.linear and cafe_amd.interact; activations in dense_dtype, the result float32."""
+        t = self.dense_dtype
+        dense = dense.to(t) if self.dense_dim else None
+        if self.kind == "dlrm":
+            x = run_mlp(self.bot_l, dense) if self.dense_dim else None
+            return run_mlp(self.top_l, dot_interaction(x, emb, self.interaction_itself, dtype=t)).float()
+        z = emb.transpose(0, 1).reshape(emb.shape[1], -1).to(t)
+        if self.dense_dim:
+            z = torch.cat([dense, z], dim=1)
+        if self.kind == "wdl":                                    # the wide logit enters the last deep layer's launch
+            return torch.sigmoid(run_mlp(self.top_l, z, residual=linear(z, self.wide.weight, self.wide.bias)).float())
+        x1 = z
+        for i in range(self.cross_layer_n):                       # x_l w is a layer of one output
+            x1 = z * linear(x1, getattr(self, f"cross_weight_{i}").t()) + getattr(self, f"cross_bias_{i}")
+        return linear(torch.cat([run_mlp(self.top_l, z), x1], dim=1), self.last_layer.weight, self.last_layer.bias, "sigmoid").float()
 
     def forward(self, dense, emb):
         """emb: [F, B, D] -> click probability [B, 1]."""
+        if self.dense_ops == "hip":
+            return self._forward_hip(dense, emb)
         B = emb.shape[1]
         if self.kind == "dlrm":
             x = self.bot_l(dense) if self.dense_dim else None
@@ -151,7 +183,7 @@ class CafeCTRModel(nn.Module):
 
     def __init__(self, kind, counts, dim, dense_dim=13, compress_rate=0.001, hash_rate=0.3, threshold=500,
                  adjust_thres=1, alpha=1.0000005, ln_bot=None, ln_top=None, device=None, seed=123, train_cross=False,
-                 interaction_itself=False, per_field_calls=True):
+                 interaction_itself=False, per_field_calls=True, dense_ops="torch", dense_dtype=torch.float32):
         super().__init__()
         self.kind, self.dim, self.dense_dim = kind, int(dim), int(dense_dim)
         self.counts = [int(c) for c in counts]
@@ -183,7 +215,7 @@ class CafeCTRModel(nn.Module):
             self._order = torch.tensor([order.index(i) for i in range(F)], dtype=torch.long)
         dev = self.embedding.device
         self.head = CafeCTRHead(kind, len(self.counts), dim, dense_dim, ln_bot, ln_top, seed, train_cross,
-                                interaction_itself)
+                                interaction_itself, dense_ops, dense_dtype)
         self._anchor = nn.Parameter(torch.zeros(()))              # gives autograd a reason to call _Lookup.backward
         self._emb_grad = None
         self.loss_fn = nn.BCELoss(reduction="mean")               # dlrm_s_pytorch.py:462, wdl.py:425, dcn.py:433

@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import config as cfg
+from .adamw import AdamW
 from .ctr_models import CafeCTRModel
 from .data import BinaryCTRDataset
 
@@ -35,6 +36,13 @@ def parse(argv=None):
     p.add_argument("--sketch-alpha", type=float, default=1.0000005)
     p.add_argument("--mini-batch-size", type=int, default=None)
     p.add_argument("--learning-rate", type=float, default=0.1)
+    p.add_argument("--dense-ops", choices=("torch", "hip"), default="torch",
+                   help="the head's layers and interaction: stock torch ops, or the package's own launches")
+    p.add_argument("--dense-dtype", choices=("f32", "bf16", "f16"), default="f32", help="the head's type (bf16 / f16: --dense-ops hip)")
+    p.add_argument("--optimizer", choices=("sgd", "adamw", "adamw8bit"), default="sgd",
+                   help="of the dense parameters (adamw: cafe_amd.adamw); the embedding tables keep their fused SGD")
+    p.add_argument("--dense-learning-rate", type=float, default=None, help="of the dense parameters (default: --learning-rate)")
+    p.add_argument("--weight-decay", type=float, default=0.01, help="of adamw")
     p.add_argument("--num-batches", type=int, default=100)
     p.add_argument("--nepochs", type=int, default=1)
     p.add_argument("--numpy-rand-seed", type=int, default=123)
@@ -65,15 +73,24 @@ def synthetic_batches(w, dense_dim, num_batches, seed, device, start=0):
         yield x, ids, y
 
 
-def save_checkpoint(path, model, step):
-    """Model parameters + tables + the complete sketch state (every slot, scalars, free list)."""
+def make_optimizer(name, params, lr, weight_decay=0.01):
+    if name == "sgd":
+        return torch.optim.SGD(params, lr=lr)
+    return AdamW(params, lr=lr, weight_decay=weight_decay, state_bits=8 if name == "adamw8bit" else 32)
+
+
+def save_checkpoint(path, model, step, optimizer=None):
+    """Model parameters + tables + the complete sketch state (every slot, scalars, free list) + the optimizer's state, if
+    it has one (SGD without momentum has none)."""
     emb = model.embedding
+    state = optimizer.state_dict() if optimizer is not None else {"state": {}}
     torch.save({"step": int(step), "head": model.head.state_dict(), "plain": model.plain.state_dict(),
                 "weight_high": emb.weight_high.cpu(),
-                "weight_hash": [w.cpu() for w in emb.weight_hash], "sketch": emb.sketch.state_tensors()}, path)
+                "weight_hash": [w.cpu() for w in emb.weight_hash], "sketch": emb.sketch.state_tensors(),
+                **({"optimizer": state} if state["state"] else {})}, path)
 
 
-def load_checkpoint(path, model):
+def load_checkpoint(path, model, optimizer=None):
     ck = torch.load(path, map_location="cpu", weights_only=True)
     emb = model.embedding
     model.head.load_state_dict(ck["head"])
@@ -83,6 +100,8 @@ def load_checkpoint(path, model):
     for w, src in zip(emb.weight_hash, ck["weight_hash"]):
         w.copy_(src)
     emb.sketch.load_state_tensors(ck["sketch"])
+    if optimizer is not None and "optimizer" in ck:
+        optimizer.load_state_dict(ck["optimizer"])
     return int(ck["step"])
 
 
@@ -122,9 +141,11 @@ def main(argv=None):
     ln_top = [0] + [int(v) for v in a.arch_mlp_top.split("-")] if a.arch_mlp_top else None
     model = CafeCTRModel(a.model, counts, dim, dense_dim=dense_dim, compress_rate=cr, hash_rate=hr, threshold=thr,
                          adjust_thres=a.adjust_threshold, alpha=a.sketch_alpha, ln_bot=ln_bot, ln_top=ln_top, device=dev,
-                         seed=a.numpy_rand_seed, per_field_calls=not a.fused_insert)
-    opt = torch.optim.SGD(model.dense_parameters(), lr=a.learning_rate)
-    step0 = load_checkpoint(a.load_model, model) if a.load_model else 0
+                         seed=a.numpy_rand_seed, per_field_calls=not a.fused_insert, dense_ops=a.dense_ops,
+                         dense_dtype={"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[a.dense_dtype])
+    opt = make_optimizer(a.optimizer, model.dense_parameters(),
+                         a.learning_rate if a.dense_learning_rate is None else a.dense_learning_rate, a.weight_decay)
+    step0 = load_checkpoint(a.load_model, model, opt) if a.load_model else 0
     print(json.dumps({"model": a.model, "fields": len(counts), "dim": dim, "batch": batch, "hotn": model.hotn,
                       "cold_rows": int(sum(model.hash_sizes)), "ids": int(sum(counts)), "start_step": step0}), flush=True)
     step, run_loss, run_n, t0 = step0, None, 0, time.time()
@@ -153,7 +174,7 @@ def main(argv=None):
                 tl, acc = evaluate(model, (b for k, b in enumerate(tb) if k < a.test_num_batches))
                 print(f"step {step}: test loss {tl:.6f} accuracy {acc:.4f}", flush=True)
     if a.save_model:
-        save_checkpoint(a.save_model, model, step)
+        save_checkpoint(a.save_model, model, step, opt)
     return model
 
 

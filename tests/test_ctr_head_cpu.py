@@ -59,3 +59,17 @@ def test_mlp_initialisation_is_seeded_like_the_reference():
     assert isinstance(a[-1], torch.nn.Sigmoid) and isinstance(a[1], torch.nn.ReLU)     # dlrm_s_pytorch.py:243-246
     w = a[0].weight.detach().numpy()
     assert abs(w.std() - np.sqrt(2 / (4 + 8))) < 0.2
+
+
+def test_dense_side_options():
+    """The package's own dense side is asked for by name, has no CPU path, and leaves parameters and their names alone."""
+    from cafe_amd import _lib
+    for kw in (dict(dense_ops="triton"), dict(dense_dtype=torch.bfloat16), dict(dense_ops="hip", dense_dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            CafeCTRHead("wdl", 4, 8, 13, **kw)
+    a, b = CafeCTRHead("wdl", 4, 8, 13, seed=2), CafeCTRHead("wdl", 4, 8, 13, seed=2, dense_ops="hip")
+    assert a.state_dict().keys() == b.state_dict().keys()
+    assert all(torch.equal(p, q) for p, q in zip(a.top_l.parameters(), b.top_l.parameters()))
+    with pytest.raises(_lib.CafeError):
+        b(torch.rand(6, 13), torch.randn(4, 6, 8))
+    assert next(CafeCTRHead("dcn", 4, 8, 13, dense_ops="hip", dense_dtype=torch.float16).parameters()).dtype == torch.float16
