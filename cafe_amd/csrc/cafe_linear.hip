@@ -16,40 +16,49 @@ using namespace cafe;
 
 namespace {
 
-enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2, ACT_GELU = 3, ACT_SILU = 4, ACT_COUNT = 5 };
+// ACT_SLOPE: backward only, the kept values are act'(z) themselves
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2, ACT_GELU = 3, ACT_SILU = 4, ACT_COUNT = 5, ACT_SLOPE = 5 };
 
-template <int ACT> __device__ __forceinline__ float act_value(float z) {
-    if (ACT == ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if (ACT == ACT_SIGMOID) return 1.f / (1.f + expf(-z));
-    // silu and gelu: 0 where the factor beside z is below float32's range, so that -inf gives the limit and not NaN
-    if (ACT == ACT_SILU) { const float e = expf(-z); return e > 3.0e38f ? 0.f : z / (1.f + e); }
-    if (ACT == ACT_GELU) {                                              // z Phi(z), no cancellation in the left tail
-        const float t = erfcf(z * -0.70710678f);
-        return t == 0.f ? 0.f : 0.5f * z * t;
+// act(z), and act'(z) where SLOPE.  relu is told by the sign alone, so its output serves as z in the backward.
+// gelu and silu: products with a factor below float32's range are 0, so that infinities give the limits and not NaN.
+template <int ACT, bool SLOPE> __device__ __forceinline__ float activate(float z, float *slope) {
+    if (ACT == ACT_RELU) {
+        if (SLOPE) *slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
+        return z > 0.f ? z : (z != z ? z : 0.f);
     }
+    if (ACT == ACT_SIGMOID || ACT == ACT_SILU) {
+        const float e = expf(-fabsf(z)), q = 1.f / (1.f + e), small = e * q;      // sigmoid(|z|), sigmoid(-|z|)
+        const float s = z > 0.f ? q : small, t = z > 0.f ? small : q;             // sigmoid(z), sigmoid(-z)
+        if (ACT == ACT_SIGMOID) {
+            if (SLOPE) *slope = q * small;
+            return z != z ? z : s;
+        }
+        if (SLOPE) *slope = small == 0.f ? s : s + z * s * t;
+        return s == 0.f ? 0.f : z * s;
+    }
+    if (ACT == ACT_GELU) {                                                        // z Phi(z), no cancellation in the left tail
+        const float phi = 0.5f * erfcf(z * -0.70710678f);
+        if (SLOPE) {
+            const float d = 0.39894228f * expf(-0.5f * z * z);
+            *slope = phi + (d == 0.f ? 0.f : z * d);
+        }
+        return phi == 0.f ? 0.f : z * phi;
+    }
+    if (SLOPE) *slope = 1.f;
     return z;
 }
-// act'(z); relu is told by the sign alone, so its kept output serves as z
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-    if (ACT == ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
-    if (ACT == ACT_SIGMOID || ACT == ACT_SILU) {
-        const float e = expf(-fabsf(z)), q = 1.f / (1.f + e);
-        const float small = e * q;                                      // sigmoid(-|z|)
-        if (ACT == ACT_SIGMOID) return q * small;
-        const float s = z > 0.f ? q : small, t = z > 0.f ? small : q;   // sigmoid(z), sigmoid(-z)
-        return small == 0.f ? s : s + z * s * t;                        // +-inf: the limits 1 and 0
-    }
-    if (ACT == ACT_GELU) {
-        const float d = 0.39894228f * expf(-0.5f * z * z);
-        return 0.5f * erfcf(z * -0.70710678f) + (d == 0.f ? 0.f : z * d);
-    }
-    return 1.f;
+// act'(z) from what was kept
+template <int ACT> __device__ __forceinline__ float act_slope(float kept) {
+    if (ACT == ACT_SLOPE) return kept;
+    float s;
+    activate<ACT, true>(kept, &s);
+    return s;
 }
 
 // Where a product's result goes.  part != null: float32 partial sums of one slice of the reduction, joined by k_join.
 struct Out {
     void *y; int64_t ldy;
-    void *kept; int64_t ldk;          // value before the activation, in the output's type (null: not wanted)
+    void *kept; int64_t ldk;          // act'(z), in the output's type (null: not wanted)
     const void *bias;
     const void *res; int64_t ldr;
     float *part;
@@ -207,11 +216,16 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
     }
 };
 
-// One result: bias, the value kept for the backward, activation, residual.
+// One result: bias, activation, its slope (kept for the backward), residual.
 template <class T, int ACT> __device__ __forceinline__ void finish(const Out &o, int64_t i, int64_t j, float v, float bias) {
     v += bias;
-    if (o.kept) ((T *)o.kept)[i * o.ldk + j] = (T)v;
-    v = act_value<ACT>(v);
+    if (o.kept) {
+        float s;
+        v = activate<ACT, true>(v, &s);
+        ((T *)o.kept)[i * o.ldk + j] = (T)s;
+    } else {
+        v = activate<ACT, false>(v, nullptr);
+    }
     if (o.res) v += (float)((const T *)o.res)[i * o.ldr + j];
     ((T *)o.y)[i * o.ldy + j] = (T)v;
 }
@@ -410,6 +424,7 @@ template <class F> void with_act(int act, F f) {
         case ACT_SIGMOID: f(std::integral_constant<int, ACT_SIGMOID>{}); break;
         case ACT_GELU: f(std::integral_constant<int, ACT_GELU>{}); break;
         case ACT_SILU: f(std::integral_constant<int, ACT_SILU>{}); break;
+        case ACT_SLOPE: f(std::integral_constant<int, ACT_SLOPE>{}); break;
         default: f(std::integral_constant<int, ACT_NONE>{}); break;
     }
 }
@@ -457,14 +472,14 @@ BwdWs bwd_ws(int64_t M, int64_t K, int64_t N, int dtype, int act) {
     return w;
 }
 
-bool bad_sizes(const char *who, int64_t m, int64_t k, int64_t n, int dtype, int act) {
+bool bad_sizes(const char *who, int64_t m, int64_t k, int64_t n, int dtype, int act, int acts = ACT_COUNT) {
     const int64_t most = INT32_MAX;
     if (m < 0 || k < 0 || n < 0 || m > most || k > most || n > most) {
         set_error("%s: sizes %lld x %lld x %lld outside 0 .. 2^31 - 1", who, (long long)m, (long long)k, (long long)n);
         return true;
     }
     if (dtype < kF32 || dtype > kF16) { set_error("%s: unknown type code %d", who, dtype); return true; }
-    if (act < 0 || act >= ACT_COUNT) { set_error("%s: unknown activation code %d", who, act); return true; }
+    if (act < 0 || act >= acts) { set_error("%s: unknown activation code %d", who, act); return true; }
     return false;
 }
 
@@ -512,7 +527,7 @@ extern "C" int64_t cafe_linear_fwd_ws(int64_t m, int64_t k, int64_t n, int dtype
 }
 
 extern "C" int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype, int act) {
-    if (bad_sizes("cafe_linear_bwd_ws", m, k, n, dtype, act)) return -1;
+    if (bad_sizes("cafe_linear_bwd_ws", m, k, n, dtype, act, ACT_SLOPE + 1)) return -1;
     return bwd_ws(m, k, n, dtype, act).bytes;
 }
 
@@ -536,7 +551,7 @@ extern "C" int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w
 extern "C" int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw,
                                    const void *d_kept, int64_t ldk, void *d_dx, int64_t lddx, void *d_dw, void *d_db, int64_t m, int64_t k,
                                    int64_t n, int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream) {
-    if (bad_sizes("cafe_linear_bwd_dev", m, k, n, dtype, act)) return 1;
+    if (bad_sizes("cafe_linear_bwd_dev", m, k, n, dtype, act, ACT_SLOPE + 1)) return 1;
     if (m > 0 && n > 0 && (!d_dy || (act != ACT_NONE && !d_kept))) { set_error("cafe_linear_bwd_dev: null gradient or kept values"); return 1; }
     if ((d_dx && m > 0 && n > 0 && k > 0 && !d_w) || (d_dw && m > 0 && n > 0 && k > 0 && !d_x)) { set_error("cafe_linear_bwd_dev: null operand"); return 1; }
     if (lddy < 0 || ldx < 0 || ldw < 0 || ldk < 0 || (d_dx && lddx < k)) { set_error("cafe_linear_bwd_dev: bad row stride"); return 1; }

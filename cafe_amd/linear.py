@@ -8,6 +8,8 @@ wide part's logit to the deep part's last activation).  Here a layer is
 on the matrix units (cafe_amd/csrc/cafe_linear.hip), float32, bfloat16 or float16, sums in float32.  `linear` is
 differentiable; `linear_forward` / `linear_backward` are the same two passes for a training step that is written out;
 `run_mlp` sends an nn.Sequential of Linear and activation modules through `linear`."""
+from typing import NamedTuple
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -16,6 +18,12 @@ from . import _lib
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2, "gelu": 3, "silu": 4}
+_SLOPE = 5
+
+
+class Slope(NamedTuple):
+    """What a forward keeps for its backward: the activation's slopes act'(z), in x's type."""
+    values: torch.Tensor
 
 
 def on_device(t):
@@ -66,7 +74,8 @@ def _check(x, weight, bias, activation, residual):
 
 
 def _forward(x, weight, bias, act, residual, keep):
-    """x [M, K], residual [M, N] or None.  Returns (y, kept): kept is what the backward needs, or None."""
+    """x [M, K], residual [M, N] or None.  Returns (y, kept): the activation's slopes; y itself for relu without a
+    residual; None without an activation or where not asked for."""
     L = _lib.load()
     x, ldx = _rows(x)
     weight, ldw = _rows(weight)
@@ -95,6 +104,7 @@ def _forward(x, weight, bias, act, residual, keep):
 
 
 def _backward(grad, x, weight, kept, act, need):
+    """act: the code that says what `kept` holds (include/cafe_hip.h, cafe_linear_bwd_dev)."""
     L = _lib.load()
     grad, ldg = _rows(grad)
     x, ldx = _rows(x)
@@ -123,7 +133,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         y, kept = _forward(x, weight, bias, act, residual, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, kept)
-        ctx.act, ctx.has_res = act, residual is not None
+        ctx.act, ctx.has_res = act if act <= ACTIVATIONS["relu"] else _SLOPE, residual is not None
         return y
 
     @staticmethod
@@ -144,7 +154,7 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     all float32, bfloat16 or float16, on one GPU.  activation: "none", "relu", "sigmoid", "gelu" (z Phi(z)) or "silu".
     Rows may be strided views.  Runs on the current stream of x's device.  Differentiable once in x, weight, bias and
     residual; the backward keeps x, weight and, for every activation but relu without a residual, one more [..., N]
-    tensor of x's type (the value before the activation)."""
+    tensor of x's type (the activation's slopes)."""
     _check(x, weight, bias, activation, residual)
     lead = x.shape[:-1]
     n = weight.shape[0]
@@ -160,29 +170,34 @@ def linear(x, weight, bias=None, activation="none", residual=None):
 
 
 def linear_forward(x, weight, bias=None, activation="none", residual=None):
-    """`linear` without autograd for x [M, K]: (y, kept), kept being what linear_backward asks for (None for "none";
-    y itself for "relu" without a residual; else the value before the activation, in x's type)."""
+    """`linear` without autograd for x [M, K]: (y, kept), kept being what linear_backward asks for (None for "none"; a
+    tensor for "relu": y itself, or the slopes where a residual hides its sign; else a Slope)."""
     _check(x, weight, bias, activation, residual)
     if x.dim() != 2:
         raise ValueError(f"x [M, K] expected, not {tuple(x.shape)}")
     if residual is not None and residual.shape != (x.shape[0], weight.shape[0]):
         raise ValueError(f"residual {tuple(residual.shape)}, the output is {(x.shape[0], weight.shape[0])}")
     with torch.no_grad():
-        return _forward(x, weight, bias, ACTIVATIONS[activation], residual, True)
+        y, kept = _forward(x, weight, bias, ACTIVATIONS[activation], residual, True)
+    return y, kept if ACTIVATIONS[activation] <= ACTIVATIONS["relu"] else Slope(kept)
 
 
 def linear_backward(grad, x, weight, kept=None, activation="none", need=(True, True, True)):
     """(dx, dweight, dbias) for the gradient of the output, grad [M, N]; None in the place of what `need` declines.
-    kept: as linear_forward returned it (for "relu" any tensor with the sign of the value before the activation)."""
+    kept: as linear_forward returned it, or a tensor [M, N] of the values before the activation (for "relu" any tensor
+    of their sign)."""
     _check(x, weight, None, activation, grad)
     shape = (x.shape[0], weight.shape[0])
     if x.dim() != 2 or tuple(grad.shape) != shape:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit grad {tuple(grad.shape)}")
-    if activation != "none":
+    act = ACTIVATIONS[activation]
+    if isinstance(kept, Slope):
+        kept, act = kept.values, _SLOPE
+    if act:
         if kept is None or tuple(kept.shape) != shape or kept.dtype != x.dtype or kept.device != x.device:
             raise ValueError(f"activation {activation!r} needs the kept [M, N] values of its forward, in x's type and on its device")
     with torch.no_grad():
-        return _backward(grad, x, weight, kept, ACTIVATIONS[activation], tuple(need))
+        return _backward(grad, x, weight, kept, act, tuple(need))
 
 
 _ACTIVATION_OF = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}

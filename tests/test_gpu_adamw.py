@@ -4,6 +4,7 @@ parameters against the formula in float64.
 Tolerance of a parameter: keep, step size, betas and eps are float32 numbers and the update is four float32 operations
 with a square root and a division, each half a step: 16 2^-24 of the update's magnitude, 4 2^-24 of the parameter, then
 half a step of the parameter's type."""
+import gc
 import math
 
 import pytest
@@ -264,6 +265,7 @@ def test_captured_step(bits):
         opt.step()
     torch.cuda.current_stream().wait_stream(side)
     ref.step()
+    gc.collect()                     # a collected model frees device memory, which a capture forbids
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         opt.step()

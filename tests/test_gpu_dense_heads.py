@@ -1,7 +1,7 @@
 """The heads on the package's own dense side (CafeCTRHead / CafeCTRModel with dense_ops="hip"): the same losses as torch's
 heads, the layers' calls in their order, training with AdamW eagerly, from a checkpoint and captured in a graph."""
 import copy
-import io
+import gc
 import os
 import sys
 
@@ -215,6 +215,7 @@ def test_a_captured_training_step(kind, bits):
         step(h1, o1, emb)
     torch.cuda.current_stream().wait_stream(side)
     step(h2, o2, e2)
+    gc.collect()                                                # a collected model frees device memory, which a capture forbids
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = step(h1, o1, emb)

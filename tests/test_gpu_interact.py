@@ -3,6 +3,8 @@
 Tolerances: a float32 sum of n products is off by at most (2 n + 16) 2^-24 times the sum of their magnitudes (the matrix
 units may order and align partial products in their own way); rounding to a type is half a step, eps / 2 relative, plus
 half the smallest subnormal."""
+import gc
+
 import pytest
 import torch
 
@@ -182,6 +184,7 @@ def test_graph_and_streams():
     with torch.cuda.stream(side):
         step()
     torch.cuda.current_stream().wait_stream(side)
+    gc.collect()                     # a collected model frees device memory, which a capture forbids
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got = step()

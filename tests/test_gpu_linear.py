@@ -5,11 +5,13 @@ to first order; the matrix units may add partial products in an order (and with 
 activation or its slope is evaluated in float32 to within 2^-20 absolute for unit arguments (a few ulp of exp and erfc);
 gelu and silu have slopes below 1.2 and second derivatives below 1.  Rounding to the output type is half a step, eps / 2
 relative, plus half the smallest subnormal."""
+import gc
+
 import pytest
 import torch
 import torch.nn as nn
 
-from cafe_amd.linear import linear, linear_backward, linear_forward, run_mlp
+from cafe_amd.linear import Slope, linear, linear_backward, linear_forward, run_mlp
 
 pytestmark = pytest.mark.gpu
 U32 = 2.0 ** -24
@@ -62,16 +64,21 @@ def check_forward(y, kept, x, w, b, r, act):
     ez = sum_error(xd, wd, k) + 4 * U32 * z.abs()
     y0 = value(z, act) + (r.double() if r is not None else 0)
     check(y, y0, 1.2 * ez + 2 ** -20 * (1 + z.abs()) * (act not in ("none", "relu")) + 4 * U32 * y0.abs() + half_step(t) * 1.01 * y0.abs() + tiny(t), "y")
-    if kept is not None and kept is not y:
-        check(kept, z, ez + half_step(t) * 1.01 * z.abs() + tiny(t), "kept")
+    if kept is not None and kept is not y:                      # act'(z); relu's: 0 or 1 by the sign, which z's error may turn
+        k = kept.values if isinstance(kept, Slope) else kept
+        s = slope(z, act)
+        off = ez + 2 ** -20 * (1 + z.abs()) if act != "relu" else (z.abs() <= ez).double()
+        check(k, s, off + half_step(t) * 1.01 * s.abs() + tiny(t), "kept")
 
 
 def check_backward(grads, dy, x, w, kept, act):
     t, m, n = x.dtype, x.shape[0], w.shape[0]
     dyd, xd, wd = dy.double(), x.double(), w.double()
-    s = slope(kept.double(), act) if act != "none" else torch.ones_like(dyd)
+    given = isinstance(kept, Slope)
+    s = kept.values.double() if given else slope(kept.double(), act) if act != "none" else torch.ones_like(dyd)
     dz = dyd * s
-    ez = dyd.abs() * (2 ** -20 if act not in ("none", "relu") else 0) + dz.abs() * 2 * U32     # float32 value
+    # float32 value; slopes that come as they are cost the product's rounding alone
+    ez = dyd.abs() * (0 if given or act in ("none", "relu") else 2 ** -20 * (1 + kept.double().abs())) + dz.abs() * 2 * U32
     rz = ez + (half_step(t) * 1.01 * dz.abs() + tiny(t) if act not in ("none", "relu") else 0)   # rounded before the products
     dx, dw, db = grads
     for got, want, err, what in (
@@ -95,6 +102,8 @@ def test_forward_and_backward(m, k, n, t):
         check_forward(y, kept, x, w, b, r, act)
         assert torch.equal(y, linear(x, w, b, act, r))
         check_backward(linear_backward(dy, x, w, kept, act), dy, x, w, kept, act)
+        z = torch.randn(m, n, device="cuda").to(t)              # from the values before the activation
+        check_backward(linear_backward(dy, x, w, z, act), dy, x, w, z, act)
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -246,6 +255,7 @@ def test_graph_capture_and_replay(t):
         with torch.cuda.stream(side):
             step(act)
         torch.cuda.current_stream().wait_stream(side)
+        gc.collect()                     # a collected model frees device memory, which a capture forbids
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out = step(act)

@@ -54,7 +54,7 @@ def test_c_entry_points():
     for m, k, n, t in ((-1, 1, 1, 0), (1, -1, 1, 0), (1, 1, 1 << 31, 0), (1, 1, 1, 3), (1, 1, 1, -1)):
         assert L.cafe_linear_fwd_ws(m, k, n, t) == -1
         assert L.cafe_linear_bwd_ws(m, k, n, t, 0) == -1
-    assert L.cafe_linear_bwd_ws(1, 1, 1, 0, 5) == -1
+    assert L.cafe_linear_bwd_ws(1, 1, 1, 0, 6) == -1 and L.cafe_linear_bwd_ws(1, 1, 1, 0, -1) == -1
     for t in range(3):                                          # every size that may be 0 has a workspace size
         for m in (0, 1, 70, 70000):
             for k in (0, 1, 5000):
@@ -65,7 +65,7 @@ def test_c_entry_points():
         return L.cafe_linear_fwd_dev(x, ldx, w, ldw, None, res, ldr, y, ldy, kept, ldk, m, k, n, t, act, ws, size, None)
 
     for kw in (dict(x=None), dict(w=None), dict(y=None), dict(ldy=6), dict(ldx=-1), dict(ldw=-5), dict(ldr=-1), dict(kept=p, ldk=6),
-               dict(m=-1), dict(t=7), dict(act=9), dict(m=64, k=1 << 20, n=64, ldx=1 << 20, ldw=1 << 20, ldy=64, size=-1)):
+               dict(m=-1), dict(t=7), dict(act=5), dict(act=9), dict(m=64, k=1 << 20, n=64, ldx=1 << 20, ldw=1 << 20, ldy=64, size=-1)):
         assert fwd(**kw) != 0, kw
         assert L.cafe_last_error()
     assert fwd(m=0, x=None, w=None, y=None) == 0                # nothing to do
@@ -74,5 +74,5 @@ def test_c_entry_points():
         return L.cafe_linear_bwd_dev(dy, lddy, x, 5, w, 5, kept, ldk, dx, lddx, dw, db, m, k, n, 0, act, ws, size, None)
 
     for kw in (dict(dy=None), dict(kept=None), dict(x=None), dict(w=None), dict(lddx=4), dict(lddy=-1), dict(ldk=-1), dict(size=0),
-               dict(ws=None), dict(act=-1), dict(k=-3)):
+               dict(ws=None), dict(act=-1), dict(act=6), dict(k=-3)):
         assert bwd(**kw) != 0, kw
