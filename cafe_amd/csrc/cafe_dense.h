@@ -26,13 +26,16 @@ template <class T> struct Elem {
 template <class T> __device__ __forceinline__ u32x4 load16(const T *p) { return ((const Chunk<sizeof(T)> *)p)->v; }
 template <class T> __device__ __forceinline__ void store16(T *p, u32x4 v) { ((Chunk<sizeof(T)> *)p)->v = v; }
 
-// chunk moved down by `n` elements, zeros behind (n >= the chunk's length: all zeros)
+// chunk moved down by `n` elements, zeros behind (n up to the chunk's length: all zeros); selects, no branches
 template <class T> __device__ __forceinline__ u32x4 shift_down(u32x4 v, int n) {
-    const int bits = n * 8 * (int)sizeof(T);
-    uint64_t lo = (uint64_t)v.x | ((uint64_t)v.y << 32), hi = (uint64_t)v.z | ((uint64_t)v.w << 32);
-    if (bits >= 64) { lo = bits >= 128 ? 0 : hi >> (bits - 64); hi = 0; }
-    else if (bits > 0) { lo = (lo >> bits) | (hi << (64 - bits)); hi >>= bits; }
-    return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    const int bits = n * 8 * (int)sizeof(T), s = bits & 63;
+    const uint64_t lo = (uint64_t)v.x | ((uint64_t)v.y << 32), hi = (uint64_t)v.z | ((uint64_t)v.w << 32);
+    uint64_t a = bits & 64 ? hi : lo, b = bits & 64 ? 0 : hi;
+    a = bits & 128 ? 0 : a;
+    b = bits & 128 ? 0 : b;
+    a = (a >> s) | ((b << 1) << (63 - s));
+    b >>= s;
+    return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
 }
 
 // the first `n` elements at p (n may be <= 0 or exceed the chunk), zeros behind; nothing past them is read

@@ -10,7 +10,13 @@
 // forward, dz in dx) or across it ("columns": W in dx; dz and x in dW).  One tile kernel serves them; see k_tile.
 #include "cafe_dense.h"
 
+#include <math.h>
+#include <stdlib.h>
+
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include <utility>
 
 using namespace cafe;
 
@@ -47,18 +53,19 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ float activate(float z
     if (SLOPE) *slope = 1.f;
     return z;
 }
-// act'(z) from what was kept
-template <int ACT> __device__ __forceinline__ float act_slope(float kept) {
-    if (ACT == ACT_SLOPE) return kept;
+// dy * act'(z) from what was kept.  Where nothing passes (relu, a slope of 0), nothing of dy does, not even an infinity.
+template <int ACT> __device__ __forceinline__ float through(float dy, float kept) {
+    if (ACT == ACT_RELU) return kept > 0.f ? dy : (kept != kept ? kept : 0.f);
+    if (ACT == ACT_SLOPE) return kept == 0.f ? 0.f : dy * kept;
     float s;
     activate<ACT, true>(kept, &s);
-    return s;
+    return dy * s;
 }
 
 // Where a product's result goes.  part != null: float32 partial sums of one slice of the reduction, joined by k_join.
 struct Out {
     void *y; int64_t ldy;
-    void *kept; int64_t ldk;          // act'(z), in the output's type (null: not wanted)
+    float *kept; int64_t ldk;         // act'(z), unrounded (null: not wanted)
     const void *bias;
     const void *res; int64_t ldr;
     float *part;
@@ -69,6 +76,7 @@ struct TileArgs {
     const void *a, *b;
     int64_t lda, ldb;
     int64_t I, J, R;                  // C is [I, J], the reduction runs over R
+    float *sums; void *sums_out;      // column sums of A: per slice, or (one slice) the result itself; null: not wanted
     int tiles_j, tiles;               // tiles along j, tiles in all
     int slices;                       // slices of the reduction (grid.y)
     Out o;
@@ -81,11 +89,23 @@ template <> __device__ __forceinline__ f32x16 mfma32<__bf16>(u32x4 a, u32x4 b, f
 template <> __device__ __forceinline__ f32x16 mfma32<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-template <> __device__ __forceinline__ f32x16 mfma32<float>(u32x4 a, u32x4 b, f32x16 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+// TI x TJ blocks of one step: 16 bytes of reduction per lane on either side.  float32 takes four products per 16 bytes;
+// they go round the accumulators, so that neighbours do not depend on each other.
+template <class T, int TI, int TJ> __device__ __forceinline__ void mfma_step(const u32x4 *a, const u32x4 *b, f32x16 (*acc)[TJ]) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[q], y[q], c, 0, 0, 0);
-    return c;
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int i = 0; i < TI; i++)
+#pragma unroll
+                for (int j = 0; j < TJ; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i][q]), __uint_as_float(b[j][q]), acc[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int j = 0; j < TJ; j++) acc[i][j] = mfma32<T>(a[i], b[j], acc[i][j]);
+    }
 }
 template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
 template <> __device__ __forceinline__ f32x4 mfma16<__bf16>(u32x4 a, u32x4 b, f32x4 c) {
@@ -104,18 +124,18 @@ template <> __device__ __forceinline__ f32x4 mfma16<float>(u32x4 a, u32x4 b, f32
 // One operand of a tile: BX entries (rows i or j) times BK = 128 bytes' worth of reduction, in LDS.
 //   rows (COLS = false):   LDS [BX][128 B + 16 B].  36 banks from row to row: the eight lanes that a 16-byte read serves
 //                          together fall on 32 different banks.
-//   columns (COLS = true): LDS [BK][BX + pad], as it lies in memory.  float32 reads one value per lane (the two half
-//                          waves are 4 rows apart: pad 8 puts them on different halves of the banks); 16-bit types read
-//                          through the transposing LDS read, 4 rows x 16 columns per 16 lanes: the row stride is 16 or
-//                          48 banks modulo 64, so the 4 rows fall on different banks.
+//   columns (COLS = true): LDS [BK][BX + 32 B], as it lies in memory.  float32 reads one value per lane (the two half waves
+//                          are 4 rows apart, on different halves of the banks); 16-bit types read through the transposing
+//                          LDS read, 4 rows x 16 columns per 16 lanes, the rows 8 (or 24, 40) banks apart.
 // A lane's fragment for step s holds the reductions 2s+h (h = lane / 32) chunk of 16 bytes in both layouts.
+// What lies outside the operand reads as 0; nothing outside is touched: a chunk that would cross a row's end is read
+// further back and shifted.
 template <class T, bool COLS, int BX, int THREADS> struct Operand {
     static constexpr int E = Elem<T>::per_chunk;
     static constexpr int BK = 8 * E;
     static constexpr int CPR = COLS ? BX / E : 8;                          // 16-byte chunks per LDS row
     static constexpr int ROWS = COLS ? BK : BX;
-    static constexpr int PAD = !COLS ? 16 : sizeof(T) == 4 ? 32 : BX == 32 ? 0 : 64;
-    static constexpr int STRIDE = CPR * 16 + PAD;                          // bytes
+    static constexpr int STRIDE = CPR * 16 + (COLS ? 32 : 16);             // bytes
     static constexpr int BYTES = ROWS * STRIDE;
     static constexpr int N = ROWS * CPR / THREADS;                         // chunks per thread
     static constexpr int STEP = THREADS / CPR;                             // rows between a thread's chunks
@@ -123,12 +143,10 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
 
     const T *p[N];           // first tile's chunks, clamped into the operand
     int64_t adv;             // elements from one tile to the next
-    int shift;               // elements to shift a chunk that was moved back to stay inside its row (columns)
-    int cols;                // contiguous extent of the operand (columns: of j; rows: of the reduction)
+    int shift;               // columns: elements to shift a chunk that was moved back to stay inside its row
+    bool tiny;               // a row is shorter than a chunk: element by element
     int64_t R, X, ld, x0;
     const T *base;
-    bool tiny;
-    u32x4 reg[N];
 
     __device__ __forceinline__ void init(const void *src, int64_t ld_, int64_t X_, int64_t R_, int64_t x0_) {
         base = (const T *)src; ld = ld_; X = X_; R = R_; x0 = x0_;
@@ -153,20 +171,24 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
             }
         }
     }
-    // Requests tile kt.  `last`: the tile that holds the end of the reduction.  What lies outside the operand reads as 0;
-    // nothing outside is touched: a chunk that would cross a row's end is read further back and shifted.
-    __device__ __forceinline__ void load(int64_t kt, bool last) {
+    __device__ __forceinline__ bool edge() const { return COLS && x0 + BX > X; }       // columns end inside this tile
+    // Requests tile kt, which lies inside the operand.
+    __device__ __forceinline__ void load_inner(u32x4 (&reg)[N], int64_t kt) const {
+#pragma unroll
+        for (int n = 0; n < N; n++) reg[n] = load16(p[n] + kt * adv);
+    }
+    // Requests tile kt.  `last`: the tile that holds the end of the reduction.
+    __device__ __forceinline__ void load(u32x4 (&reg)[N], int64_t kt, bool last) const {
         const int t = threadIdx.x, c = t % CPR, row = t / CPR;
-        if (tiny) {
+        if (!last && !(COLS && tiny)) {
+            load_inner(reg, kt);
+        } else if (tiny) {
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 const int64_t r = row + n * STEP;
                 if (COLS) reg[n] = kt * BK + r < R ? load_some(base + (kt * BK + r) * ld + x0 + c * E, (int)(X - x0 - c * E)) : u32x4{0, 0, 0, 0};
                 else { const int64_t k = kt * BK + c * E; reg[n] = k < R ? load_some(p[n] + kt * BK, (int)(R - k)) : u32x4{0, 0, 0, 0}; }
             }
-        } else if (!last) {
-#pragma unroll
-            for (int n = 0; n < N; n++) reg[n] = load16(p[n] + kt * adv);
         } else if (COLS) {
 #pragma unroll
             for (int n = 0; n < N; n++) {
@@ -188,14 +210,16 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
             }
         }
     }
-    __device__ __forceinline__ void store(char *lds) const {
+    __device__ __forceinline__ void align(u32x4 (&reg)[N]) const {
+        if (edge() && !tiny) {
+#pragma unroll
+            for (int n = 0; n < N; n++) reg[n] = shift_down<T>(reg[n], shift);
+        }
+    }
+    __device__ __forceinline__ static void store(const u32x4 (&reg)[N], char *lds) {
         const int t = threadIdx.x, c = t % CPR, row = t / CPR;
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            u32x4 v = reg[n];
-            if (COLS && shift && !tiny) v = shift_down<T>(v, shift);
-            *(u32x4 *)(lds + (row + n * STEP) * STRIDE + c * 16) = v;
-        }
+        for (int n = 0; n < N; n++) *(u32x4 *)(lds + (row + n * STEP) * STRIDE + c * 16) = reg[n];
     }
     // fragment of the 32 entries from x (within the tile) for step s
     __device__ __forceinline__ static u32x4 frag(const char *lds, int x, int s) {
@@ -216,35 +240,65 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
     }
 };
 
-// One result: bias, activation, its slope (kept for the backward), residual.
-template <class T, int ACT> __device__ __forceinline__ void finish(const Out &o, int64_t i, int64_t j, float v, float bias) {
-    v += bias;
+// `left` results of one row from column j: bias, activation, its slope (kept for the backward), residual.
+template <class T, int ACT> __device__ __forceinline__ void finish(const Out &o, int64_t i, int64_t j, float *v, const float *bias, int left) {
+    constexpr int E = Elem<T>::per_chunk;
+    float s[E], r[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) r[e] = 0.f;
+    if (o.res) unpack<T>(load_some((const T *)o.res + i * o.ldr + j, left), r);
     if (o.kept) {
-        float s;
-        v = activate<ACT, true>(v, &s);
-        ((T *)o.kept)[i * o.ldk + j] = (T)s;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = activate<ACT, true>(v[e] + bias[e], &s[e]);
+#pragma unroll
+        for (int h = 0; h < E; h += 4) store_some(o.kept + i * o.ldk + j + h, pack<float>(s + h), left - h);
     } else {
-        v = activate<ACT, false>(v, nullptr);
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = activate<ACT, false>(v[e] + bias[e], nullptr);
     }
-    if (o.res) v += (float)((const T *)o.res)[i * o.ldr + j];
-    ((T *)o.y)[i * o.ldy + j] = (T)v;
+    if (o.res) {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] += r[e];
+    }
+    store_some((T *)o.y + i * o.ldy + j, pack<T>(v), left);
+}
+template <class T> __device__ __forceinline__ void bias_chunk(const Out &o, int64_t j, int left, float *b) {
+#pragma unroll
+    for (int e = 0; e < Elem<T>::per_chunk; e++) b[e] = 0.f;
+    if (o.bias) unpack<T>(load_some((const T *)o.bias + j, left), b);
 }
 
-// C tile of BM x BN by WM x WN waves, each (BM / WM) x (BN / WN) in 32 x 32 MFMA blocks.
-template <class T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64) void k_tile(TileArgs g) {
-    constexpr int TH = WM * WN * 64, TI = BM / WM / 32, TJ = BN / WN / 32;
-    typedef Operand<T, ACOLS, BM, TH> OA;
-    typedef Operand<T, BCOLS, BN, TH> OB;
-    constexpr int BK = OA::BK;
-    __shared__ __align__(16) char lds[OA::BYTES + OB::BYTES];
-    char *la = lds, *lb = lds + OA::BYTES;
+// Order of issue for the scheduler: MF products with R LDS reads, W LDS writes and V memory reads spread between them.  A
+// wave issues in order: eight writes in a row hold it until LDS has taken them, while the matrix unit runs dry.
+template <int MF, int R, int W, int V, int I> __device__ __forceinline__ void weave_one() {
+    constexpr int T = R + W + V, m = (I + 1) * MF / T - I * MF / T;
+    if constexpr (m > 0) __builtin_amdgcn_sched_group_barrier(0x8, m, 0);
+    __builtin_amdgcn_sched_group_barrier(I < R ? 0x100 : I < R + W ? 0x200 : 0x20, 1, 0);
+}
+template <int MF, int R, int W, int V, int... I> __device__ __forceinline__ void weave_all(std::integer_sequence<int, I...>) {
+    (weave_one<MF, R, W, V, I>(), ...);
+}
+template <int MF, int R, int W, int V> __device__ __forceinline__ void weave() {
+    weave_all<MF, R, W, V>(std::make_integer_sequence<int, R + W + V>{});
+}
+
+// C tile of BM x BN by four waves in 2 x 2, each (BM / 2) x (BN / 2) in 32 x 32 MFMA blocks.  Two LDS buffers, one barrier
+// per 128 bytes of reduction: a wave that writes buffer k % 2 has passed the barrier behind every read of it.  PF tiles
+// are on their way in registers: a float32 tile computes for longer than memory takes to answer (64 products of 64
+// cycles per wave), a 16-bit one (16 of 32) does not.
+template <class T, bool ACOLS, bool BCOLS, int BM, int BN>
+__global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
+    constexpr int TI = BM / 64, TJ = BN / 64, E = Elem<T>::per_chunk, PF = sizeof(T) == 4 ? 1 : 2;
+    typedef Operand<T, ACOLS, BM, 256> OA;
+    typedef Operand<T, BCOLS, BN, 256> OB;
+    constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, CS = BN + 8;
+    __shared__ __align__(16) char lds[2 * STAGE > BM * CS * 4 ? 2 * STAGE : BM * CS * 4];
     const int tile = xcd_tile(blockIdx.x, g.tiles);
     const int64_t i0 = (int64_t)(tile / g.tiles_j) * BM, j0 = (int64_t)(tile % g.tiles_j) * BN;
     const int64_t kts = (g.R + BK - 1) / BK;
     const int64_t k0 = kts * blockIdx.y / g.slices, k1 = kts * (blockIdx.y + 1) / g.slices;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
+    const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
     f32x16 acc[TI][TJ];
 #pragma unroll
     for (int a = 0; a < TI; a++)
@@ -252,59 +306,164 @@ __global__ __launch_bounds__(WM *WN * 64) void k_tile(TileArgs g) {
         for (int b = 0; b < TJ; b++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[a][b][e] = 0.f;
-    OA A; OB B;
+    OA A;
+    OB B;
     A.init(g.a, g.lda, g.I, g.R, i0);
     B.init(g.b, g.ldb, g.J, g.R, j0);
-    if (k0 < k1) { A.load(k0, k0 == kts - 1); B.load(k0, k0 == kts - 1); }
-    for (int64_t kt = k0; kt < k1; kt++) {
-        A.store(la); B.store(lb);
+    u32x4 ra[PF][OA::N], rb[PF][OB::N];
+    const bool sums = ACOLS && BCOLS && g.sums && j0 == 0;
+    float cs[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) cs[e] = 0.f;
+
+    auto request = [&](int64_t kt, int u, bool inner) {
+        if (inner) {
+            A.load_inner(ra[u], kt);
+            B.load_inner(rb[u], kt);
+        } else {
+            const bool last = kt == kts - 1;
+            A.load(ra[u], kt, last);
+            B.load(rb[u], kt, last);
+        }
+    };
+    // Registers of set u -> LDS buffer of tile kt.
+    auto stage = [&](int64_t kt, int u, bool woven) {
+        char *la = lds + (kt & 1) * STAGE, *lb = la + OA::BYTES;
+        if (!woven) { A.align(ra[u]); B.align(rb[u]); }
+        if (!woven && sums) {
+#pragma unroll
+            for (int n = 0; n < OA::N; n++) {
+                float v[E];
+                unpack<T>(ra[u][n], v);
+#pragma unroll
+                for (int e = 0; e < E; e++) cs[e] += v[e];
+            }
+        }
+        OA::store(ra[u], la);
+        OB::store(rb[u], lb);
+    };
+    u32x4 fa[2][TI], fb[2][TJ];
+    auto fetch = [&](int64_t kt, int s, int f) {
+        const char *la = lds + (kt & 1) * STAGE, *lb = la + OA::BYTES;
+#pragma unroll
+        for (int a = 0; a < TI; a++) fa[f][a] = OA::frag(la, wi + 32 * a, s);
+#pragma unroll
+        for (int b = 0; b < TJ; b++) fb[f][b] = OB::frag(lb, wj + 32 * b, s);
+    };
+    // Tile kt: its first fragments are in set 0.  The next tile goes to LDS behind step 1, the barrier stands behind step
+    // 2, and the next tile's first fragments are fetched before step 3's products: the matrix unit always has a step's
+    // worth of work while LDS answers.
+    // INNER: every tile it touches lies inside the operands and the slice; WOVEN: nor has a chunk to be shifted or a column
+    // to be summed, so that no branch stands between the products.
+    constexpr int MF = TI * TJ * (sizeof(T) == 4 ? 4 : 1), FR = TI * (ACOLS ? 2 : 1) + TJ * (BCOLS ? 2 : 1), MV = OA::N + OB::N;
+    auto body = [&](int64_t kt, int u, auto mode) {
+        constexpr bool INNER = decltype(mode)::value > 0, WOVEN = decltype(mode)::value == 2;
+        const int un = (u + 1) % PF;
+        fetch(kt, 1, 1);
+        if (INNER || kt + 1 < k1) stage(kt + 1, un, WOVEN);
+        mfma_step<T, TI, TJ>(fa[0], fb[0], acc);
+        if constexpr (WOVEN) weave<MF, FR, MV, 0>();
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(kt, 2, 0);
+        if (INNER || kt + 1 + PF < k1) request(kt + 1 + PF, un, INNER);
+        mfma_step<T, TI, TJ>(fa[1], fb[1], acc);
+        if constexpr (WOVEN) weave<MF, FR, 0, MV>();
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(kt, 3, 1);
+        mfma_step<T, TI, TJ>(fa[0], fb[0], acc);
+        if constexpr (WOVEN) weave<MF, FR, 0, 0>();
         __syncthreads();
-        if (kt + 1 < k1) { A.load(kt + 1, kt + 1 == kts - 1); B.load(kt + 1, kt + 1 == kts - 1); }
+        if (INNER || kt + 1 < k1) fetch(kt + 1, 0, 0);
+        mfma_step<T, TI, TJ>(fa[1], fb[1], acc);
+    };
+    if (k0 < k1) {
+        const bool woven = !(sums || A.edge() || B.edge());
+        // tiles that the inner bodies may request: all but the reduction's last, none where rows are shorter than a chunk
+        const int64_t inner = A.tiny || B.tiny ? k0 : k1 < kts ? k1 : kts - 1;
+        int64_t kt = k0;
+        auto start = [&](auto mode) {
+            constexpr bool IN = decltype(mode)::value > 0;
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            u32x4 fa[TI], fb[TJ];
+            for (int u = 0; u < PF; u++)
+                if (IN || k0 + u < k1) {
+                    request(k0 + u, u, IN);
+                    __builtin_amdgcn_sched_barrier(0);          // in this order: the loop waits for the older set
+                }
+            stage(k0, 0, decltype(mode)::value == 2);
+            if (IN || k0 + PF < k1) request(k0 + PF, 0, IN);
+            __syncthreads();
+            fetch(k0, 0, 0);
+        };
+        auto run = [&](auto mode) {
+            start(mode);
+            for (; kt + 2 * PF < inner; kt += PF) {
 #pragma unroll
-            for (int a = 0; a < TI; a++) fa[a] = OA::frag(la, wi + 32 * a, s);
+                for (int u = 0; u < PF; u++) body(kt + u, u, mode);
+            }
+        };
+        if (k0 + 2 * PF >= inner) start(std::integral_constant<int, 0>{});
+        else if (woven) run(std::integral_constant<int, 2>{});
+        else if constexpr (ACOLS || BCOLS) run(std::integral_constant<int, 1>{});
+        for (; kt < k1; kt += PF) {
 #pragma unroll
-            for (int b = 0; b < TJ; b++) fb[b] = OB::frag(lb, wj + 32 * b, s);
-#pragma unroll
-            for (int a = 0; a < TI; a++)
-#pragma unroll
-                for (int b = 0; b < TJ; b++) acc[a][b] = mfma32<T>(fa[a], fb[b], acc[a][b]);
+            for (int u = 0; u < PF; u++)
+                if (kt + u < k1) body(kt + u, u, std::integral_constant<int, 0>{});
+        }
+    }
+    __syncthreads();
+
+    // The tile goes through LDS, so that a thread ends up with neighbouring columns of a row: 16-byte accesses to
+    // everything that follows.  Accumulator element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
+    float *c = (float *)lds;
+    if (sums) {                                 // 256 / CPR threads hold partial sums of the same columns
+        for (int e = 0; e < E; e++) c[threadIdx.x * E + e] = cs[e];
+        __syncthreads();
+        if (threadIdx.x < BM && i0 + threadIdx.x < g.I) {
+            float v = 0.f;
+            for (int q = 0; q < OA::STEP; q++) v += c[q * BM + threadIdx.x];
+            if (g.sums_out) ((T *)g.sums_out)[i0 + threadIdx.x] = (T)v;
+            else g.sums[blockIdx.y * g.I + i0 + threadIdx.x] = v;
         }
         __syncthreads();
     }
-    // accumulator element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32
-    const int lj = lane & 31, li = 4 * (lane >> 5);
+    if (!g.o.part && !g.o.y) return;
+#pragma unroll
+    for (int a = 0; a < TI; a++)
+#pragma unroll
+        for (int b = 0; b < TJ; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                c[(wi + 32 * a + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * CS + wj + 32 * b + (lane & 31)] = acc[a][b][e];
+    __syncthreads();
+    constexpr int CH = BN / E, PASS = BM * CH / 256;
+    const int col = threadIdx.x % CH * E;
+    const int64_t j = j0 + col;
+    const int left = (int)(g.J - j < E ? g.J - j : E);
+    if (left <= 0) return;
     if (g.o.part) {
         float *part = g.o.part + (int64_t)blockIdx.y * g.I * g.J;
+#pragma unroll 2
+        for (int q = 0; q < PASS; q++) {
+            const int row = threadIdx.x / CH + q * (256 / CH);
+            const int64_t i = i0 + row;
+            if (i >= g.I) break;
 #pragma unroll
-        for (int a = 0; a < TI; a++)
-#pragma unroll
-            for (int b = 0; b < TJ; b++) {
-                const int64_t j = j0 + wj + 32 * b + lj;
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int64_t i = i0 + wi + 32 * a + 8 * (e >> 2) + li + (e & 3);
-                    if (i < g.I && j < g.J) part[i * g.J + j] = acc[a][b][e];
-                }
-            }
+            for (int h = 0; h < E; h += 4) store_some(part + i * g.J + j + h, *(const u32x4 *)(c + row * CS + col + h), left - h);
+        }
         return;
     }
+    float bias[E];
+    bias_chunk<T>(g.o, j, left, bias);
     auto put = [&](auto actc) {
-        constexpr int ACT = decltype(actc)::value;
+#pragma unroll 2
+        for (int q = 0; q < PASS; q++) {
+            const int row = threadIdx.x / CH + q * (256 / CH);
+            const int64_t i = i0 + row;
+            if (i >= g.I) break;
+            float v[E];
 #pragma unroll
-        for (int b = 0; b < TJ; b++) {
-            const int64_t j = j0 + wj + 32 * b + lj;
-            if (j >= g.J) continue;
-            const float bias = g.o.bias ? (float)((const T *)g.o.bias)[j] : 0.f;
-#pragma unroll
-            for (int a = 0; a < TI; a++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int64_t i = i0 + wi + 32 * a + 8 * (e >> 2) + li + (e & 3);
-                    if (i < g.I) finish<T, ACT>(g.o, i, j, acc[a][b][e], bias);
-                }
+            for (int e = 0; e < E; e++) v[e] = c[row * CS + col + e];
+            finish<T, decltype(actc)::value>(g.o, i, j, v, bias, left);
         }
     };
     if (!ACOLS && !BCOLS) {
@@ -320,68 +479,156 @@ __global__ __launch_bounds__(WM *WN * 64) void k_tile(TileArgs g) {
     }
 }
 
-// Sum of the reduction's slices in their order, then what follows the product.
-template <class T, int ACT> __global__ __launch_bounds__(256) void k_join(Out o, int64_t I, int64_t J, int slices) {
-    const int64_t n = I * J;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
-        float v = 0.f;
-        for (int s = 0; s < slices; s++) v += o.part[s * n + q];
-        const int64_t i = q / J, j = q - i * J;
-        finish<T, ACT>(o, i, j, v, o.bias ? (float)((const T *)o.bias)[j] : 0.f);
-    }
-}
-
-// dz = dy * act'(kept), and the column sums of dz over this block's rows (float32, from the unrounded products).
-// A thread holds one 16-byte chunk of columns; blockDim = lanes_x chunks x 256 / lanes_x rows.
+// Sum of the reduction's slices in their order, then what follows the product; the blocks behind `out_blocks` join the
+// column sums.
 template <class T, int ACT>
-__global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const T *kept, int64_t ldk, T *dz, int64_t M, int N,
-                                           int lanes_x, int64_t rows, float *sums) {
+__global__ __launch_bounds__(256) void k_join(Out o, int64_t I, int64_t J, int slices, int out_blocks, const float *sums, T *sums_out) {
     constexpr int E = Elem<T>::per_chunk;
-    __shared__ float red[256 * E];
-    const int lx = threadIdx.x % lanes_x, ly = threadIdx.x / lanes_x, ny = 256 / lanes_x;
-    const int64_t col = ((int64_t)blockIdx.x * lanes_x + lx) * E;
-    const int left = (int)(N - col < E ? N - col : E);
-    const int64_t m0 = blockIdx.y * rows, m1 = m0 + rows < M ? m0 + rows : M;
-    float s[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) s[e] = 0.f;
-    if (left > 0)
-        for (int64_t m = m0 + ly; m < m1; m += ny) {
-            float g[E];
-            unpack<T>(load_some(dy + m * ldy + col, left), g);
-            if (ACT != ACT_NONE) {
-                float k[E];
-                unpack<T>(load_some(kept + m * ldk + col, left), k);
-#pragma unroll
-                for (int e = 0; e < E; e++) g[e] *= act_slope<ACT>(k[e]);
-                store_some(dz + m * N + col, pack<T>(g), left);
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) s[e] += g[e];
-        }
-    if (!sums) return;
-#pragma unroll
-    for (int e = 0; e < E; e++) red[threadIdx.x * E + e] = s[e];
-    __syncthreads();
-    for (int w = threadIdx.x; w < lanes_x * E; w += 256) {
-        const int64_t c = (int64_t)blockIdx.x * lanes_x * E + w;
-        if (c >= N) continue;
+    if ((int)blockIdx.x >= out_blocks) {
+        const int64_t i = (int64_t)(blockIdx.x - out_blocks) * 256 + threadIdx.x;
+        if (i >= I) return;
         float v = 0.f;
-        for (int y = 0; y < ny; y++) v += red[y * lanes_x * E + w];
-        sums[blockIdx.y * (int64_t)N + c] = v;
+#pragma unroll 8
+        for (int s = 0; s < slices; s++) v += sums[s * I + i];
+        sums_out[i] = (T)v;
+        return;
+    }
+    const int64_t chunks = (J + E - 1) / E, n = I * chunks;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)out_blocks * 256) {
+        const int64_t i = q / chunks, j = (q - i * chunks) * E;
+        const int left = (int)(J - j < E ? J - j : E);
+        float v[E], bias[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = 0.f;
+        const float *part = o.part + i * J + j;
+        constexpr int AHEAD = 32 / E;           // slices on their way at a time; added in their order
+        int s = 0;
+        for (; s + AHEAD <= slices && left >= E; s += AHEAD) {
+            u32x4 w[AHEAD][E / 4];
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+                for (int h = 0; h < E / 4; h++) w[u][h] = load16(part + (s + u) * (I * J) + 4 * h);
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] += __uint_as_float(w[u][e / 4][e % 4]);
+        }
+        for (; s < slices; s++)
+#pragma unroll
+            for (int h = 0; h < E / 4; h++) {
+                const u32x4 w = load_some(part + s * (I * J) + 4 * h, left - 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * h + e] += __uint_as_float(w[e]);
+            }
+        bias_chunk<T>(o, j, left, bias);
+        finish<T, ACT>(o, i, j, v, bias, left);
     }
 }
 
-// db: the blocks' column sums in their order.  64 columns x 4 runs of blocks per workgroup.
-template <class T> __global__ __launch_bounds__(256) void k_db(const float *sums, int blocks, int N, T *db) {
-    __shared__ float red[256];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), y = threadIdx.x >> 6;
-    float v = 0.f;
-    if (c < N)
-        for (int b = blocks * y / 4; b < blocks * (y + 1) / 4; b++) v += sums[(int64_t)b * N + c];
-    red[threadIdx.x] = v;
+// y = act(x W^T + b) + r where one side has at most 64 rows (a few samples, or a layer of a few outputs).  Nothing is
+// shared between workgroups but the few rows, and there is too little work to fill tiles: a workgroup takes 16 rows of the
+// long side (`many`) against all of the short one (FT groups of 16), its WAVES waves take turns along the reduction, and
+// operands go from memory to the matrix unit without LDS: lane l holds 16 bytes of row l % 16, chunk l / 16 of the step's
+// four, which is the fragment of a 16 x 16 product.  The waves' sums are added through LDS in their order.
+// MANY_W: the long side is W (rows of y are the short side's).
+struct SkinnyArgs {
+    const void *many, *few;
+    int64_t ldm, ldf;
+    int64_t M, N, K;                  // of the layer
+    Out o;
+};
+
+template <class T, int FT, int WAVES, bool MANY_W> __global__ __launch_bounds__(WAVES * 64) void k_skinny(SkinnyArgs g) {
+    constexpr int E = Elem<T>::per_chunk, STEP = 4 * E, U = FT <= 2 ? 4 : 2;
+    __shared__ float part[WAVES][FT * 4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int64_t many = MANY_W ? g.N : g.M, few = MANY_W ? g.M : g.N, K = g.K;
+    const int64_t i0 = (int64_t)blockIdx.x * 16;
+    const T *pa = (const T *)g.many + (i0 + r < many ? i0 + r : many - 1) * g.ldm + q * E;
+    const T *pb[FT];
+#pragma unroll
+    for (int f = 0; f < FT; f++) pb[f] = (const T *)g.few + (16 * f + r < few ? 16 * f + r : few - 1) * g.ldf + q * E;
+    f32x4 acc[FT];
+#pragma unroll
+    for (int f = 0; f < FT; f++) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t whole = K / STEP;                 // steps that lie inside the rows
+    int64_t s = wave;
+    for (; s + (U - 1) * WAVES < whole; s += U * WAVES) {
+        u32x4 a[U], b[U][FT];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] = load16(pa + (s + u * WAVES) * STEP);
+#pragma unroll
+            for (int f = 0; f < FT; f++) b[u][f] = load16(pb[f] + (s + u * WAVES) * STEP);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int f = 0; f < FT; f++) acc[f] = mfma16<T>(a[u], b[u][f], acc[f]);
+    }
+    for (; s * STEP < K; s += WAVES) {
+        const int left = (int)(K - s * STEP - q * E < E ? K - s * STEP - q * E : E);
+        const u32x4 a = load_some(pa + s * STEP, left);
+        u32x4 b[FT];
+#pragma unroll
+        for (int f = 0; f < FT; f++) b[f] = load_some(pb[f] + s * STEP, left);
+#pragma unroll
+        for (int f = 0; f < FT; f++) acc[f] = mfma16<T>(a, b[f], acc[f]);
+    }
+#pragma unroll
+    for (int f = 0; f < FT; f++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) part[wave][f * 4 + e][lane] = acc[f][e];
     __syncthreads();
-    if (y == 0 && c < N) db[c] = (T)(red[threadIdx.x] + red[64 + threadIdx.x] + red[128 + threadIdx.x] + red[192 + threadIdx.x]);
+    // accumulator element e of lane l: long row 4 (l / 16) + e, short row l % 16 of its group
+    auto put = [&](auto actc) {
+        constexpr int ACT = decltype(actc)::value;
+        for (int t = threadIdx.x; t < 256 * FT; t += WAVES * 64) {
+            const int i = MANY_W ? t & 15 : (t >> 4) & 15, j = MANY_W ? t >> 4 : (t & 15) + 16 * (t >> 8);
+            if (i0 + i >= many || j >= few) continue;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) v += part[w][(j >> 4) * 4 + (i & 3)][16 * (i >> 2) + (j & 15)];
+            const int64_t m = MANY_W ? j : i0 + i, n = MANY_W ? i0 + i : j;
+            if (g.o.bias) v += (float)((const T *)g.o.bias)[n];
+            float slope;
+            v = activate<ACT, true>(v, &slope);
+            if (g.o.kept) g.o.kept[m * g.o.ldk + n] = slope;
+            if (g.o.res) v += (float)((const T *)g.o.res)[m * g.o.ldr + n];
+            ((T *)g.o.y)[m * g.o.ldy + n] = (T)v;
+        }
+    };
+    switch (g.o.act) {
+        case ACT_RELU: put(std::integral_constant<int, ACT_RELU>{}); break;
+        case ACT_SIGMOID: put(std::integral_constant<int, ACT_SIGMOID>{}); break;
+        case ACT_GELU: put(std::integral_constant<int, ACT_GELU>{}); break;
+        case ACT_SILU: put(std::integral_constant<int, ACT_SILU>{}); break;
+        default: put(std::integral_constant<int, ACT_NONE>{}); break;
+    }
+}
+
+// dz = dy * act'(z), rounded.  kept: z in the type (relu: anything of its sign), or the slopes in float32.  One 16-byte
+// chunk per thread and step.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t M, int64_t N) {
+    constexpr int E = Elem<T>::per_chunk;
+    const int64_t chunks = (N + E - 1) / E, n = M * chunks;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
+        const int64_t m = q / chunks, col = (q - m * chunks) * E;
+        const int left = (int)(N - col < E ? N - col : E);
+        float g[E], k[E];
+        unpack<T>(load_some(dy + m * ldy + col, left), g);
+        if constexpr (ACT == ACT_SLOPE) {
+#pragma unroll
+            for (int h = 0; h < E; h += 4) unpack<float>(load_some((const float *)kept + m * ldk + col + h, left - h), k + h);
+        } else {
+            unpack<T>(load_some((const T *)kept + m * ldk + col, left), k);
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) g[e] = through<ACT>(g[e], k[e]);
+        store_some(dz + m * N + col, pack<T>(g), left);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -390,30 +637,53 @@ template <class T> __global__ __launch_bounds__(256) void k_db(const float *sums
 int64_t elem_size(int dtype) { return dtype == kF32 ? 4 : 2; }
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Tile and slices of a product.
-struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; };
+// Tile and slices of a product: the smallest estimate of its time, in microseconds,
+//
+//     steps x max(alone, load x shared) + load x ends + join
+//
+// steps: 128-byte steps of the reduction per slice; load: workgroups per compute unit; shared, alone: what a step costs
+// a compute unit among workgroups that fill it and in one that runs by itself (128 x 128, one side 64, 64 x 64); ends:
+// loading the first tile and storing the result; join: the second launch, the way of the partial sums out and back
+// (2.5 TB/s) and the slices.  The constants are fitted to 1500 timings of 45 products between 1 x 256 x 8192 and 16384 x
+// 3341 x 256 in float32 and bfloat16; the choice is within 1.2 % of the fastest on average and 27 % off at worst (1 x 256
+// outputs over 8192 in bfloat16).  Both sides of it: 8192 x 256 outputs over 512 in bfloat16 take 8.0 us in 64 x 64 tiles
+// and 10.5 in 128 x 128 (half the units idle), 8192 x 1024 over 1024 take 30.8 and 25.0; 64 x 256 outputs over 8192 in
+// float32 take 14.7 us in 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and 11.9 in 12.
+struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; double us; };
+struct Cost { double shared[3], alone[3], ends, join, per_slice, launch; };
 
 Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
-    Plan p;
-    const int64_t bk = 128 / elem_size(dtype), kts = std::max<int64_t>(1, (R + bk - 1) / bk);
-    p.bm = I > 64 ? 128 : 64;
-    p.bn = J > 64 ? 128 : 64;
-    auto count = [&]() { p.tiles_i = (I + p.bm - 1) / p.bm; p.tiles_j = (J + p.bn - 1) / p.bn; p.tiles = p.tiles_i * p.tiles_j; };
-    count();
-    if (p.tiles < 256) { p.bm = p.bn = 64; count(); }
-    p.slices = 1;
-    if (p.tiles > 0 && p.tiles < 256) p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({512 / p.tiles, kts / 4, 64}));
-    p.ws = p.slices > 1 ? up256((int64_t)p.slices * I * J * 4) : 0;
-    return p;
+    static const Cost f32 = {{1.82, 1.0, 0.535}, {2.32, 1.18, 0.65}, 2.5, 1.7, 0.065, 4.7};
+    static const Cost half = {{0.585, 0.43, 0.28}, {0.80, 0.56, 0.31}, 1.7, 2.3, 0.14, 4.4};
+    const Cost &c = dtype == kF32 ? f32 : half;
+    const int64_t bk = 128 / elem_size(dtype), kts = (R + bk - 1) / bk;
+    Plan best = {};
+    double least = 0;
+    for (int bm = 128; bm >= 64; bm /= 2)
+        for (int bn = 128; bn >= 64; bn /= 2) {
+            const int kind = (bm == 64) + (bn == 64);
+            const int64_t ti = (I + bm - 1) / bm, tj = std::max<int64_t>(1, (J + bn - 1) / bn);
+            for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64}) {
+                if (s > 1 && (ti * tj * s > 2048 || kts < 2 * s)) break;
+                const double load = std::ceil((double)ti * tj * s / 256.0), steps = (double)((kts + s - 1) / s);
+                double t = steps * std::max(c.alone[kind], c.shared[kind] * load) + c.ends * load * (bm * bn) / 16384.0;
+                if (s > 1) t += c.join + c.per_slice * s + 4e-7 * 4 * s * (double)I * J;
+                if (best.bm == 0 || t < least) { least = t; best = Plan{bm, bn, ti, tj, ti * tj, s, 0, t + c.launch}; }
+            }
+        }
+#ifdef CAFE_TUNE
+    if (const char *e = getenv("CAFE_TUNE_PLAN")) { sscanf(e, "%d,%d,%d", &best.bm, &best.bn, &best.slices); best.tiles_i=(I+best.bm-1)/best.bm; best.tiles_j=std::max<int64_t>(1,(J+best.bn-1)/best.bn); best.tiles=best.tiles_i*best.tiles_j; }
+#endif
+    best.ws = best.slices > 1 ? up256((int64_t)best.slices * I * J * 4) : 0;
+    return best;
 }
 
 template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, hipStream_t st) {
-    const dim3 grid((unsigned)p.tiles, (unsigned)p.slices);
-    g.tiles_j = (int)p.tiles_j; g.tiles = (int)p.tiles; g.slices = p.slices;
-    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64, 2, 2>), grid, dim3(256), 0, st, g);
-    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    const dim3 grid((unsigned)g.tiles, (unsigned)p.slices);
+    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128>), grid, dim3(256), 0, st, g);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64>), grid, dim3(256), 0, st, g);
+    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64>), grid, dim3(256), 0, st, g);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -429,46 +699,47 @@ template <class F> void with_act(int act, F f) {
     }
 }
 
-// C = A B (+ what follows) for operands of type T; `part`: workspace of p.ws bytes.
-template <class T, bool AC, bool BC> int product(const Plan &p, TileArgs g, float *part, hipStream_t st) {
-    if (g.I == 0 || g.J == 0) return 0;
-    const Out out = g.o;
-    if (p.slices > 1) g.o.part = part;
+// C = A B^T (+ what follows) for operands of type T; `part`, `sums`: workspace of p.ws and p.sums_ws bytes.  sums_out: the
+// sums of A's columns (gradient of a bias), or null.  g.o.y == null: the sums alone.
+template <class T, bool AC, bool BC> int product(const Plan &p, TileArgs g, float *part, float *sums, T *sums_out, hipStream_t st) {
+    if (g.I == 0 || (g.J == 0 && !sums_out)) return 0;
+    const bool out = g.o.y != nullptr && g.J > 0;
+    if (!out) { g.b = g.a; g.ldb = g.lda; g.J = g.I; g.o.y = nullptr; }      // one column of tiles, whose products nobody reads
+    const Out o = g.o;
+    g.tiles_j = out ? (int)p.tiles_j : 1;
+    g.tiles = (int)p.tiles_i * g.tiles_j;
+    g.slices = p.slices;
+    g.sums = sums_out ? sums : nullptr;
+    g.sums_out = p.slices == 1 ? sums_out : nullptr;
+    if (p.slices > 1 && out) g.o.part = part;
     if (launch_tile<T, AC, BC>(p, g, st)) return 1;
     if (p.slices > 1) {
-        Out o = out;
-        o.part = part;
-        const unsigned blocks = (unsigned)std::min<int64_t>((g.I * g.J + 255) / 256, 256 * 16);
-        with_act(o.act, [&](auto a) { hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3(blocks), dim3(256), 0, st, o, g.I, g.J, p.slices); });
+        Out j = o;
+        j.part = part;
+        constexpr int E = Elem<T>::per_chunk;
+        const int out_blocks = out ? (int)std::min<int64_t>((g.I * ((g.J + E - 1) / E) + 255) / 256, 256 * 16) : 0;
+        const int sum_blocks = sums_out ? (int)((g.I + 255) / 256) : 0;
+        with_act(o.act, [&](auto a) {
+            hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3((unsigned)(out_blocks + sum_blocks)), dim3(256), 0, st, j, g.I, g.J, p.slices,
+                               out_blocks, sums, sums_out);
+        });
         CAFE_HIP_CHECK(hipGetLastError());
     }
     return 0;
 }
 
-struct DzPlan { int lanes_x; int64_t blocks_x, blocks_y, rows; };
-DzPlan dz_plan(int64_t M, int64_t N, int dtype) {
-    DzPlan d;
-    const int64_t chunks = (N + 16 / elem_size(dtype) - 1) / (16 / elem_size(dtype));
-    d.lanes_x = 1;
-    while (d.lanes_x < 64 && d.lanes_x < chunks) d.lanes_x *= 2;
-    d.blocks_x = std::max<int64_t>(1, (chunks + d.lanes_x - 1) / d.lanes_x);
-    const int64_t ny = 256 / d.lanes_x;
-    const int64_t want = std::max<int64_t>(1, 1024 / d.blocks_x);
-    d.rows = std::max<int64_t>(ny, (M + want - 1) / want);
-    d.rows = (d.rows + ny - 1) / ny * ny;
-    d.blocks_y = std::max<int64_t>(1, (M + d.rows - 1) / d.rows);
-    return d;
-}
+// dz is formed once, rounded to the type, ahead of both products.  Formed in their loads instead (dy times the slopes, two
+// operands read in place of one) it cost float32 more than it saved: 321 us against 307 at 8192 x 1024 x 1024; 16-bit
+// types would read both once per column of tiles.
 
-// workspace of the backward: [dz][column sums][partial products, used by dx, then by dW]
-struct BwdWs { int64_t dz, sums, part, bytes; };
+// workspace of the backward: [dz][column sums of the slices][partial products, used by dx, then by dW]
+struct BwdWs { int64_t sums, part, bytes; };
 BwdWs bwd_ws(int64_t M, int64_t K, int64_t N, int dtype, int act) {
     BwdWs w;
-    const DzPlan d = dz_plan(M, N, dtype);
-    w.dz = 0;
+    const Plan dx = plan(M, K, N, dtype), dw = plan(N, K, M, dtype);
     w.sums = act == ACT_NONE ? 0 : up256(M * N * elem_size(dtype));
-    w.part = w.sums + up256(d.blocks_y * N * 4);
-    w.bytes = w.part + std::max(plan(M, K, N, dtype).ws, plan(N, K, M, dtype).ws);
+    w.part = w.sums + up256((int64_t)dw.slices * N * 4);
+    w.bytes = w.part + std::max(dx.ws, dw.ws);
     return w;
 }
 
@@ -483,38 +754,72 @@ bool bad_sizes(const char *who, int64_t m, int64_t k, int64_t n, int dtype, int 
     return false;
 }
 
+template <class T, int FT, bool MANY_W> int launch_skinny(const SkinnyArgs &g, hipStream_t st) {
+    const int64_t many = MANY_W ? g.N : g.M;
+    const unsigned blocks = (unsigned)((many + 15) / 16);
+    if (many <= 16 * 512) hipLaunchKernelGGL((k_skinny<T, FT, 8, MANY_W>), dim3(blocks), dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_skinny<T, FT, 4, MANY_W>), dim3(blocks), dim3(256), 0, st, g);
+    CAFE_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+template <class T, bool MANY_W> int skinny(const SkinnyArgs &g, hipStream_t st) {
+    const int64_t few = MANY_W ? g.M : g.N;
+    if (few <= 16) return launch_skinny<T, 1, MANY_W>(g, st);
+    if (few <= 32) return launch_skinny<T, 2, MANY_W>(g, st);
+    return launch_skinny<T, 4, MANY_W>(g, st);
+}
+// Estimate of k_skinny's time, in microseconds: the waves' way along a row (a memory latency per batch of loads, dearer with
+// every short row; four times that where 16-bit rows start at odd addresses: 1 x 3341 x 1024 in bfloat16 takes 11.9 us,
+// 1 x 3344 x 1024 takes 4.6) or the rows' way from memory.  At 1 x 479 x 1024 it takes 4.6 us in bfloat16 (the tiles 6.6),
+// at 8192 x 256 x 1 in float32 4.2 (the tiles 9.5), at 64 x 1024 x 1024 in float32 12.8 (the tiles 9.7).
+double skinny_us(int64_t m, int64_t k, int64_t n, int dtype, bool aligned) {
+    const double few = (double)std::min(m, n), many = (double)std::max(m, n), row = (double)k * elem_size(dtype);
+    return 2.9 + std::max(row * (0.0005 + 0.000025 * few) * (aligned ? 1 : 4), many * row * (aligned ? 1 : 2) * (1 + few / 64) / 5e6);
+}
+bool is_skinny(int64_t m, int64_t k, int64_t n, int dtype, bool aligned) {
+    return std::min(m, n) <= 64 && skinny_us(m, k, n, dtype, aligned) < plan(m, n, k, dtype).us;
+}
+
 template <class T> int fwd(TileArgs g, void *ws, int dtype, hipStream_t st) {
-    return product<T, false, false>(plan(g.I, g.J, g.R, dtype), g, (float *)ws, st);
+    const bool aligned = sizeof(T) == 4 || (((g.lda | g.ldb) & 1) == 0 && (((uintptr_t)g.a | (uintptr_t)g.b) & 3) == 0);
+    if (is_skinny(g.I, g.R, g.J, dtype, aligned)) {
+        if (g.I <= g.J) return skinny<T, true>(SkinnyArgs{g.b, g.a, g.ldb, g.lda, g.I, g.J, g.R, g.o}, st);
+        return skinny<T, false>(SkinnyArgs{g.a, g.b, g.lda, g.ldb, g.I, g.J, g.R, g.o}, st);
+    }
+    return product<T, false, false>(plan(g.I, g.J, g.R, dtype), g, (float *)ws, nullptr, nullptr, st);
+}
+int64_t fwd_ws(int64_t m, int64_t k, int64_t n, int dtype) {
+    return is_skinny(m, k, n, dtype, dtype == kF32) ? 0 : plan(m, n, k, dtype).ws;      // whatever the alignment turns out to be
 }
 
 template <class T>
-int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t ldw, const T *kept, int64_t ldk, T *dx, int64_t lddx,
+int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t ldw, const void *kept, int64_t ldk, T *dx, int64_t lddx,
         T *dw, T *db, int64_t M, int64_t K, int64_t N, int dtype, int act, char *ws, hipStream_t st) {
     const BwdWs at = bwd_ws(M, K, N, dtype, act);
+    float *sums = (float *)(ws + at.sums), *part = (float *)(ws + at.part);
     const T *dz = dy;
     int64_t lddz = lddy;
-    float *sums = (float *)(ws + at.sums), *part = (float *)(ws + at.part);
-    const DzPlan d = dz_plan(M, N, dtype);
-    if (N > 0 && (act != ACT_NONE || db)) {
-        T *z = act != ACT_NONE ? (T *)(ws + at.dz) : nullptr;
-        with_act(act, [&](auto a) {
-            hipLaunchKernelGGL((k_dz<T, decltype(a)::value>), dim3((unsigned)d.blocks_x, (unsigned)d.blocks_y), dim3(256), 0, st, dy, lddy,
-                               kept, ldk, z, M, (int)N, d.lanes_x, d.rows, db ? sums : nullptr);
-        });
+    if (act != ACT_NONE && M > 0 && N > 0 && (dx || dw || db)) {
+        T *z = (T *)ws;
+        constexpr int E = Elem<T>::per_chunk;
+        const unsigned blocks = (unsigned)std::min<int64_t>((M * ((N + E - 1) / E) + 255) / 256, 256 * 32);
+        with_act(act, [&](auto a) { hipLaunchKernelGGL((k_dz<T, decltype(a)::value>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, M, N); });
         CAFE_HIP_CHECK(hipGetLastError());
-        if (z) { dz = z; lddz = N; }
-        if (db) {
-            hipLaunchKernelGGL(k_db<T>, dim3((unsigned)((N + 63) / 64)), dim3(256), 0, st, sums, (int)d.blocks_y, (int)N, db);
-            CAFE_HIP_CHECK(hipGetLastError());
-        }
+        dz = z; lddz = N;
     }
+    TileArgs g = {};
+    g.a = dz; g.lda = lddz;
     if (dx) {
-        TileArgs g = {dz, w, lddz, ldw, M, K, N, 0, 0, 1, {dx, lddx, nullptr, 0, nullptr, nullptr, 0, nullptr, ACT_NONE}};
-        if (product<T, false, true>(plan(M, K, N, dtype), g, part, st)) return 1;
+        TileArgs q = g;
+        q.b = w; q.ldb = ldw; q.I = M; q.J = K; q.R = N;
+        q.o.y = dx; q.o.ldy = lddx;
+        if (product<T, false, true>(plan(M, K, N, dtype), q, part, nullptr, nullptr, st)) return 1;
     }
-    if (dw) {
-        TileArgs g = {dz, x, lddz, ldx, N, K, M, 0, 0, 1, {dw, K, nullptr, 0, nullptr, nullptr, 0, nullptr, ACT_NONE}};
-        if (product<T, true, true>(plan(N, K, M, dtype), g, part, st)) return 1;
+    if (dw || db) {
+        TileArgs q = g;
+        q.b = x; q.ldb = ldx; q.I = N; q.J = K; q.R = M;
+        q.o.y = dw; q.o.ldy = K;
+        return product<T, true, true>(plan(N, K, M, dtype), q, part, sums, db, st);
     }
     return 0;
 }
@@ -523,7 +828,7 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
 
 extern "C" int64_t cafe_linear_fwd_ws(int64_t m, int64_t k, int64_t n, int dtype) {
     if (bad_sizes("cafe_linear_fwd_ws", m, k, n, dtype, 0)) return -1;
-    return plan(m, n, k, dtype).ws;
+    return fwd_ws(m, k, n, dtype);
 }
 
 extern "C" int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype, int act) {
@@ -532,18 +837,20 @@ extern "C" int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype
 }
 
 extern "C" int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, const void *d_res,
-                                   int64_t ldr, void *d_y, int64_t ldy, void *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
+                                   int64_t ldr, void *d_y, int64_t ldy, float *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
                                    int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream) {
     if (bad_sizes("cafe_linear_fwd_dev", m, k, n, dtype, act)) return 1;
     if (m == 0 || n == 0) return 0;
     if (!d_y || (k > 0 && (!d_x || !d_w))) { set_error("cafe_linear_fwd_dev: null pointer"); return 1; }
     if (ldx < 0 || ldw < 0 || ldr < 0 || ldy < n || (d_kept && ldk < n)) { set_error("cafe_linear_fwd_dev: bad row stride"); return 1; }
-    const int64_t need = plan(m, n, k, dtype).ws;
+    const int64_t need = fwd_ws(m, k, n, dtype);
     if (ws_bytes < need || (need && !d_ws)) {
         set_error("cafe_linear_fwd_dev: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
         return 1;
     }
-    TileArgs g = {d_x, d_w, ldx, ldw, m, n, k, 0, 0, 1, {d_y, ldy, d_kept, ldk, d_bias, d_res, ldr, nullptr, act}};
+    TileArgs g = {};
+    g.a = d_x; g.lda = ldx; g.b = d_w; g.ldb = ldw; g.I = m; g.J = n; g.R = k;
+    g.o = Out{d_y, ldy, d_kept, ldk, d_bias, d_res, ldr, nullptr, act};
     const hipStream_t st = (hipStream_t)stream;
     return dtype == kF32 ? fwd<float>(g, d_ws, dtype, st) : dtype == kBF16 ? fwd<__bf16>(g, d_ws, dtype, st) : fwd<_Float16>(g, d_ws, dtype, st);
 }
@@ -561,7 +868,7 @@ extern "C" int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d
         return 1;
     }
     const hipStream_t st = (hipStream_t)stream;
-#define CAFE_BWD(T) bwd<T>((const T *)d_dy, lddy, (const T *)d_x, ldx, (const T *)d_w, ldw, (const T *)d_kept, ldk, (T *)d_dx, lddx, (T *)d_dw, \
+#define CAFE_BWD(T) bwd<T>((const T *)d_dy, lddy, (const T *)d_x, ldx, (const T *)d_w, ldw, d_kept, ldk, (T *)d_dx, lddx, (T *)d_dw, \
                            (T *)d_db, m, k, n, dtype, act, (char *)d_ws, st)
     return dtype == kF32 ? CAFE_BWD(float) : dtype == kBF16 ? CAFE_BWD(__bf16) : CAFE_BWD(_Float16);
 #undef CAFE_BWD

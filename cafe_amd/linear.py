@@ -8,6 +8,7 @@ wide part's logit to the deep part's last activation).  Here a layer is
 on the matrix units (cafe_amd/csrc/cafe_linear.hip), float32, bfloat16 or float16, sums in float32.  `linear` is
 differentiable; `linear_forward` / `linear_backward` are the same two passes for a training step that is written out;
 `run_mlp` sends an nn.Sequential of Linear and activation modules through `linear`."""
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -22,7 +23,7 @@ _SLOPE = 5
 
 
 class Slope(NamedTuple):
-    """What a forward keeps for its backward: the activation's slopes act'(z), in x's type."""
+    """What a forward keeps for its backward: the activation's slopes act'(z), float32 whatever x's type."""
     values: torch.Tensor
 
 
@@ -34,19 +35,30 @@ def on_device(t):
 
 class launch_on:
     """The current stream of `t`'s device, with that device current inside the block."""
+    __slots__ = ("index", "before")
 
     def __init__(self, t):
         self.index = t.device.index
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        self.before = torch._C._cuda_getDevice()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
             torch.cuda.set_device(self.before)
+
+
+@lru_cache(maxsize=4096)
+def _fwd_ws(m, k, n, code):
+    return _lib.load().cafe_linear_fwd_ws(m, k, n, code)
+
+
+@lru_cache(maxsize=4096)
+def _bwd_ws(m, k, n, code, act):
+    return _lib.load().cafe_linear_bwd_ws(m, k, n, code, act)
 
 
 def _rows(t):
@@ -92,9 +104,9 @@ def _forward(x, weight, bias, act, residual, keep):
         if act == ACTIVATIONS["relu"] and residual is None:
             kept = y
         else:
-            kept = torch.empty_like(y)
+            kept = torch.empty(m, n, dtype=torch.float32, device=x.device)
     with launch_on(x) as st:
-        need = L.cafe_linear_fwd_ws(m, k, n, code)
+        need = _fwd_ws(m, k, n, code)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need > 0 else None
         _lib.check(L.cafe_linear_fwd_dev(x.data_ptr(), ldx, weight.data_ptr(), ldw, None if bias is None else bias.data_ptr(),
                                          rp, ldr, y.data_ptr(), n, None if kept is None or kept is y else kept.data_ptr(), n,
@@ -120,7 +132,7 @@ def _backward(grad, x, weight, kept, act, need):
     dw = new(n, k) if need[1] else None
     db = new(n) if need[2] else None
     with launch_on(x) as st:
-        size = L.cafe_linear_bwd_ws(m, k, n, code, act)
+        size = _bwd_ws(m, k, n, code, act)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size > 0 else None
         p = lambda t: None if t is None else t.data_ptr()                              # noqa: E731
         _lib.check(L.cafe_linear_bwd_dev(grad.data_ptr(), ldg, x.data_ptr(), ldx, weight.data_ptr(), ldw, kp, ldk, p(dx), k,
@@ -133,7 +145,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         y, kept = _forward(x, weight, bias, act, residual, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, kept)
-        ctx.act, ctx.has_res = act if act <= ACTIVATIONS["relu"] else _SLOPE, residual is not None
+        ctx.act, ctx.has_res = act if kept is None or kept is y else _SLOPE, residual is not None
         return y
 
     @staticmethod
@@ -154,7 +166,7 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     all float32, bfloat16 or float16, on one GPU.  activation: "none", "relu", "sigmoid", "gelu" (z Phi(z)) or "silu".
     Rows may be strided views.  Runs on the current stream of x's device.  Differentiable once in x, weight, bias and
     residual; the backward keeps x, weight and, for every activation but relu without a residual, one more [..., N]
-    tensor of x's type (the activation's slopes)."""
+    tensor, the activation's slopes in float32."""
     _check(x, weight, bias, activation, residual)
     lead = x.shape[:-1]
     n = weight.shape[0]
@@ -170,8 +182,8 @@ def linear(x, weight, bias=None, activation="none", residual=None):
 
 
 def linear_forward(x, weight, bias=None, activation="none", residual=None):
-    """`linear` without autograd for x [M, K]: (y, kept), kept being what linear_backward asks for (None for "none"; a
-    tensor for "relu": y itself, or the slopes where a residual hides its sign; else a Slope)."""
+    """`linear` without autograd for x [M, K]: (y, kept), kept being what linear_backward asks for (None for "none";
+    y itself for "relu" without a residual; else a Slope)."""
     _check(x, weight, bias, activation, residual)
     if x.dim() != 2:
         raise ValueError(f"x [M, K] expected, not {tuple(x.shape)}")
@@ -179,7 +191,7 @@ def linear_forward(x, weight, bias=None, activation="none", residual=None):
         raise ValueError(f"residual {tuple(residual.shape)}, the output is {(x.shape[0], weight.shape[0])}")
     with torch.no_grad():
         y, kept = _forward(x, weight, bias, ACTIVATIONS[activation], residual, True)
-    return y, kept if ACTIVATIONS[activation] <= ACTIVATIONS["relu"] else Slope(kept)
+    return y, kept if kept is None or kept is y else Slope(kept)
 
 
 def linear_backward(grad, x, weight, kept=None, activation="none", need=(True, True, True)):
@@ -191,11 +203,13 @@ def linear_backward(grad, x, weight, kept=None, activation="none", need=(True, T
     if x.dim() != 2 or tuple(grad.shape) != shape:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit grad {tuple(grad.shape)}")
     act = ACTIVATIONS[activation]
+    want = x.dtype
     if isinstance(kept, Slope):
-        kept, act = kept.values, _SLOPE
+        kept, act, want = kept.values, _SLOPE, torch.float32
     if act:
-        if kept is None or tuple(kept.shape) != shape or kept.dtype != x.dtype or kept.device != x.device:
-            raise ValueError(f"activation {activation!r} needs the kept [M, N] values of its forward, in x's type and on its device")
+        if kept is None or tuple(kept.shape) != shape or kept.dtype != want or kept.device != x.device:
+            raise ValueError(f"activation {activation!r} needs what its forward kept: a Slope (float32), or the values before the "
+                             f"activation in x's type, of shape {shape} on x's device")
     with torch.no_grad():
         return _backward(grad, x, weight, kept, act, tuple(need))
 

@@ -329,18 +329,18 @@ void cafe_ae_ref_update(int idx);
 /* y[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + res[M, N], all of one type, sums in float32 (dlrm_s_pytorch.py:213-251:
  * a Linear and its activation; wdl.py:704-721: the last deep layer with the wide part's logit as `res`).
  * act: 0 none, 1 relu, 2 sigmoid, 3 gelu (z Phi(z)), 4 silu.  d_bias, d_res, d_kept may be null.  d_kept [M, N] receives
- * act'(z), rounded to the type (a value near z's size would lose the slope's digits when rounded to 16 bits): what the
- * backward of sigmoid, gelu and silu needs, and relu's where `res` hides the sign of its output.  ldx, ldw and ldr may be 0 (one row repeated); ldy and ldk at least n.
+ * act'(z) in float32 (rounded to 16 bits, it would cost the gradients one more rounding than they have): what the backward
+ * of sigmoid, gelu and silu needs, and relu's where `res` hides the sign of its output.  ldx, ldw and ldr may be 0 (one row repeated); ldy and ldk at least n.
  * m, n or k may be 0 (k == 0: the sum is 0).  Workspace: cafe_linear_fwd_ws bytes (-1: bad sizes). */
 int64_t cafe_linear_fwd_ws(int64_t m, int64_t k, int64_t n, int dtype);
 int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, const void *d_res,
-                        int64_t ldr, void *d_y, int64_t ldy, void *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
+                        int64_t ldr, void *d_y, int64_t ldy, float *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
                         int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream);
 /* Gradients of the same: dz = dy * act'(kept); dx[M, K] = dz w, dw[N, K] = dz^T x (contiguous), db[N] = column sums of dz.
  * Any of d_dx, d_dw, d_db may be null (not wanted).  d_kept [M, N]: for act 2, 3, 4 the value before the activation; for
- * relu that, its output or its slope (only the sign is read); for act 5 the slope act'(z) of any activation, as the
- * forward wrote it; not read for act 0.  dz is rounded to the type before the products (they run on the
- * matrix units); db sums the unrounded values.  The result does not depend on the run: every sum has a
+ * relu that or its output (only the sign is read), of type `dtype`; for act 5 the float32 slopes act'(z) of any
+ * activation, as the forward wrote them; not read for act 0.  dz is rounded to the type before the products (they run on the
+ * matrix units); db sums the same values.  The result does not depend on the run: every sum has a
  * fixed order. */
 int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype, int act);
 int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw,

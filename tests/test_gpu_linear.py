@@ -68,7 +68,8 @@ def check_forward(y, kept, x, w, b, r, act):
         k = kept.values if isinstance(kept, Slope) else kept
         s = slope(z, act)
         off = ez + 2 ** -20 * (1 + z.abs()) if act != "relu" else (z.abs() <= ez).double()
-        check(k, s, off + half_step(t) * 1.01 * s.abs() + tiny(t), "kept")
+        assert k.dtype == torch.float32
+        check(k, s, off + 2 * U32 * s.abs(), "kept")
 
 
 def check_backward(grads, dy, x, w, kept, act):
@@ -84,7 +85,7 @@ def check_backward(grads, dy, x, w, kept, act):
     for got, want, err, what in (
             (dx, dz @ wd, rz @ wd.abs() + (2 * n + 16) * U32 * (dz.abs() @ wd.abs()), "dx"),
             (dw, dz.t() @ xd, rz.t() @ xd.abs() + (2 * m + 16) * U32 * (dz.t().abs() @ xd.abs()), "dw"),
-            (db, dz.sum(0), ez.sum(0) + (m + 16) * U32 * dz.abs().sum(0), "db")):
+            (db, dz.sum(0), rz.sum(0) + (2 * m + 16) * U32 * dz.abs().sum(0), "db")):
         if got is not None:
             check(got, want, err + half_step(t) * 1.01 * want.abs() + tiny(t), what)
 
@@ -164,7 +165,7 @@ def test_empty(t):
     check_forward(y, kept, x, w, b, r, "relu")
     dx, dw, db = linear_backward(dy, x, w, kept, "relu")
     assert dx.shape == (4, 0) and dw.shape == (7, 0)
-    check(db, (dy.double() * (kept.double() > 0)).sum(0), 8 * half_step(t) * dy.double().abs().sum(0) + tiny(t), "db")
+    check(db, (dy.double() * (kept.values > 0)).sum(0), 8 * half_step(t) * dy.double().abs().sum(0) + tiny(t), "db")
     x, w, b, r, dy = make(4, 6, 0, t)
     y, kept = linear_forward(x, w, b, "silu")
     dx, dw, db = linear_backward(dy, x, w, kept, "silu")
@@ -237,6 +238,12 @@ def test_infinities_and_nan_stay_in_their_rows(t, act):
     kept2[5, 3], kept2[6, 3] = float("inf"), float("-inf")
     dx, dw, db = linear_backward(dy, x, w, kept2, act)
     assert dx.isfinite().all() and dw.isfinite().all() and db.isfinite().all()
+    if act == "relu":                                           # an infinite gradient where nothing passes does not
+        kept2[9, 4], dy[9, 4] = -1.0, float("inf")
+        kept2[10, 4], dy[10, 4] = 0.0, float("nan")
+        for kept in (kept2, Slope((kept2 > 0).float())):
+            dx, dw, db = linear_backward(dy, x, w, kept, act)
+            assert dx.isfinite().all() and dw.isfinite().all() and db.isfinite().all()
 
 
 @pytest.mark.parametrize("t", TYPES)
