@@ -71,6 +71,22 @@ template <class T> __device__ __forceinline__ u32x4 pack(const float *f) {
     return u.v;
 }
 
+// 16 x 16 product of one 16-byte chunk per lane on either side: lane l holds row l % 16, chunk l / 16 of four.
+// Accumulator element e of lane l: row 4 (l / 16) + e of the first, row l % 16 of the second operand.
+template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 mfma16<__bf16>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma16<_Float16>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma16<float>(u32x4 a, u32x4 b, f32x4 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[q], y[q], c, 0, 0, 0);
+    return c;
+}
+
 // Workgroups are handed to the eight XCDs in turn; each XCD has its own L2.  Renumbered so that one XCD works on a
 // contiguous run of tiles (neighbours share operand rows).  A permutation of 0 .. n-1 for every n.
 __device__ __forceinline__ int xcd_tile(int id, int n) {

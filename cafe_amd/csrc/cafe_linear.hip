@@ -107,20 +107,6 @@ template <class T, int TI, int TJ> __device__ __forceinline__ void mfma_step(con
             for (int j = 0; j < TJ; j++) acc[i][j] = mfma32<T>(a[i], b[j], acc[i][j]);
     }
 }
-template <class T> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c);
-template <> __device__ __forceinline__ f32x4 mfma16<__bf16>(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ f32x4 mfma16<_Float16>(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <> __device__ __forceinline__ f32x4 mfma16<float>(u32x4 a, u32x4 b, f32x4 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[q], y[q], c, 0, 0, 0);
-    return c;
-}
-
 // One operand of a tile: BX entries (rows i or j) times BK = 128 bytes' worth of reduction, in LDS.
 //   rows (COLS = false):   LDS [BX][128 B + 16 B].  36 banks from row to row: the eight lanes that a 16-byte read serves
 //                          together fall on 32 different banks.
