@@ -24,7 +24,12 @@ using namespace cafe;
 namespace {
 
 constexpr int kItems = 48;              // tensors of one launch: their descriptors travel as kernel arguments (4 KB at most)
-constexpr int kSpan = 4096;             // values per workgroup: 4 waves x 4 blocks of 256
+// Neighbouring values per lane.  8-bit states: 8, so that codes are 8-byte accesses and 32 lanes hold a block (37 M bfloat16
+// values with master weights: 138 us; with 4 per lane 149).  float32 states: 4, 16 bytes of each array (200 us; with 8,
+// 32 bytes apart, 216).  A workgroup takes 256 times that, without a loop: enough of them are resident to hide the way
+// from memory to memory.
+constexpr int lane_values(int bits) { return bits == 8 ? 8 : 4; }
+constexpr int span(int bits) { return 256 * lane_values(bits); }
 constexpr int kBlock = 256;
 
 struct Item { void *p; const void *g; void *m, *v; uint8_t *me, *ve; float *w; int64_t n; };
@@ -37,31 +42,26 @@ struct AdamArgs {
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
-template <class T> struct Four;         // four elements, at element alignment
-template <> struct Four<float> { struct __attribute__((packed, aligned(4))) V { u32x4 v; }; };
-template <> struct Four<__bf16> { struct __attribute__((packed, aligned(2))) V { u32x2 v; }; };
-template <> struct Four<_Float16> { struct __attribute__((packed, aligned(2))) V { u32x2 v; }; };
-template <> struct Four<uint8_t> { struct __attribute__((packed, aligned(1))) V { uint32_t v; }; };
-
-template <class T, class F> __device__ __forceinline__ void get4(const T *p, int n, F *out) {
-    union { typename Four<T>::V v; T e[4]; } u;
-    if (n >= 4) {
-        u.v = *(const typename Four<T>::V *)p;
+// L elements, at element alignment, as float or int; from `n` on nothing is touched and zeros are read
+template <class T, int L> struct __attribute__((packed, aligned(sizeof(T)))) Lane { T e[L]; };
+template <int L, class T, class F> __device__ __forceinline__ void get(const T *p, int n, F *out) {
+    if (n >= L) {
+        const Lane<T, L> u = *(const Lane<T, L> *)p;
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = (F)u.e[i];
+        for (int i = 0; i < L; i++) out[i] = (F)u.e[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = i < n ? (F)p[i] : (F)0;
+        for (int i = 0; i < L; i++) out[i] = i < n ? (F)p[i] : (F)0;
     }
 }
-template <class T, class F> __device__ __forceinline__ void put4(T *p, int n, const F *in) {
-    union { typename Four<T>::V v; T e[4]; } u;
+template <int L, class T, class F> __device__ __forceinline__ void put(T *p, int n, const F *in) {
+    Lane<T, L> u;
 #pragma unroll
-    for (int i = 0; i < 4; i++) u.e[i] = (T)in[i];
-    if (n >= 4) *(typename Four<T>::V *)p = u.v;
+    for (int i = 0; i < L; i++) u.e[i] = (T)in[i];
+    if (n >= L) *(Lane<T, L> *)p = u;
     else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < L; i++)
             if (i < n) p[i] = u.e[i];
     }
 }
@@ -90,17 +90,21 @@ template <bool SECOND> __device__ __forceinline__ int encode8(float x, int e) {
     c = min(c, 0x7f);
     return x < 0.f && c > 0 ? c | 0x80 : c;
 }
-// exponent of a block of 256 values, four per lane of one wave
-__device__ __forceinline__ int block_exponent(const float *x) {
-    float top = 0.f;
+// Exponents of a block of m and of v, eight values per lane of 32 lanes.  The largest magnitude's exponent is the largest
+// exponent, so both go through the lanes as the two halves of one word (0 .. 254; what is not finite counts as 0).
+__device__ __forceinline__ void block_exponents(const float *m, const float *v, int *em, int *ev) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float mag = fabsf(x[i]);
-        if (mag <= 3.4028234663852886e38f) top = fmaxf(top, mag);
+    for (int i = 0; i < 8; i++) {
+        const uint32_t a = (__float_as_uint(m[i]) >> 23) & 255, b = (__float_as_uint(v[i]) >> 23) & 255;
+        top = __builtin_elementwise_max(top, u16x2{(unsigned short)(a == 255 ? 0 : a), (unsigned short)(b == 255 ? 0 : b)});
     }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    return max(exponent_of(top), -126);
+    for (int d = 16; d; d >>= 1)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, __shfl_xor(__builtin_bit_cast(int, top), d, 64)));
+    *em = max((int)top.x - 127, -126);
+    *ev = max((int)top.y - 127, -126);
 }
 
 __device__ __forceinline__ int item_of(const int32_t *first, int count, int block) {
@@ -117,52 +121,49 @@ template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(Ad
     const Item t = a.t[k];
     float step_size = a.step_size, root = a.root, keep = a.keep;
     if (a.factors) { step_size = a.factors[0]; root = a.factors[1]; keep = a.factors[2]; }
-    const int64_t base = (int64_t)(blockIdx.x - a.first[k]) * kSpan;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int u = 0; u < kSpan / kBlock / 4; u++) {
-        const int64_t block = base / kBlock + u * 4 + wave, at = block * kBlock + lane * 4;
-        if (block * kBlock >= t.n) return;
-        const int n = (int)(t.n - at < 4 ? t.n - at : 4);              // may be <= 0
-        float p[4], g[4], m[4], v[4];
-        get4((const T *)t.g + at, n, g);
-        if (t.w) get4(t.w + at, n, p);
-        else get4((const T *)t.p + at, n, p);
-        if (BITS8) {
-            int cm[4], cv[4];
-            get4((const uint8_t *)t.m + at, n, cm);
-            get4((const uint8_t *)t.v + at, n, cv);
-            const int em = (int)t.me[block] - 127, ev = (int)t.ve[block] - 127;
+    constexpr int BITS = BITS8 ? 8 : 32, L = lane_values(BITS);
+    const int64_t at = (int64_t)(blockIdx.x - a.first[k]) * span(BITS) + threadIdx.x * L, block = at / kBlock;
+    if (block * kBlock >= t.n) return;                  // the block's 32 lanes leave together
+    const int n = (int)(t.n - at < L ? t.n - at : L);          // may be <= 0
+    float p[L], g[L], m[L], v[L];
+    get<L>((const T *)t.g + at, n, g);
+    if (t.w) get<L>(t.w + at, n, p);
+    else get<L>((const T *)t.p + at, n, p);
+    if (BITS8) {
+        int cm[L], cv[L];
+        get<L>((const uint8_t *)t.m + at, n, cm);
+        get<L>((const uint8_t *)t.v + at, n, cv);
+        const int em = (int)t.me[block] - 127, ev = (int)t.ve[block] - 127;
 #pragma unroll
-            for (int i = 0; i < 4; i++) { m[i] = decode8<false>(cm[i], em); v[i] = decode8<true>(cv[i], ev); }
-        } else {
-            get4((const float *)t.m + at, n, m);
-            get4((const float *)t.v + at, n, v);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            m[i] = m[i] * a.b1 + g[i] * a.c1;
-            v[i] = v[i] * a.b2 + (g[i] * g[i]) * a.c2;
-            const float denom = sqrtf(v[i]) * root + a.eps;
-            p[i] = p[i] * keep - (m[i] / denom) * step_size;
-        }
-        if (BITS8) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (i >= n) m[i] = v[i] = 0.f;
-            const int em = block_exponent(m), ev = block_exponent(v);
-            int cm[4], cv[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) { cm[i] = encode8<false>(m[i], em); cv[i] = encode8<true>(v[i], ev); }
-            put4((uint8_t *)t.m + at, n, cm);
-            put4((uint8_t *)t.v + at, n, cv);
-            if (lane == 0) { t.me[block] = (uint8_t)(em + 127); t.ve[block] = (uint8_t)(ev + 127); }
-        } else {
-            put4((float *)t.m + at, n, m);
-            put4((float *)t.v + at, n, v);
-        }
-        if (t.w) put4(t.w + at, n, p);
-        put4((T *)t.p + at, n, p);
+        for (int i = 0; i < L; i++) { m[i] = decode8<false>(cm[i], em); v[i] = decode8<true>(cv[i], ev); }
+    } else {
+        get<L>((const float *)t.m + at, n, m);
+        get<L>((const float *)t.v + at, n, v);
     }
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        m[i] = m[i] * a.b1 + g[i] * a.c1;
+        v[i] = v[i] * a.b2 + (g[i] * g[i]) * a.c2;
+        const float denom = sqrtf(v[i]) * root + a.eps;
+        p[i] = p[i] * keep - (m[i] / denom) * step_size;
+    }
+    if (BITS8) {
+#pragma unroll
+        for (int i = 0; i < L; i++)
+            if (i >= n) m[i] = v[i] = 0.f;
+        int em, ev, cm[L], cv[L];
+        block_exponents(m, v, &em, &ev);
+#pragma unroll
+        for (int i = 0; i < L; i++) { cm[i] = encode8<false>(m[i], em); cv[i] = encode8<true>(v[i], ev); }
+        put<L>((uint8_t *)t.m + at, n, cm);
+        put<L>((uint8_t *)t.v + at, n, cv);
+        if ((threadIdx.x & 31) == 0) { t.me[block] = (uint8_t)(em + 127); t.ve[block] = (uint8_t)(ev + 127); }
+    } else {
+        put<L>((float *)t.m + at, n, m);
+        put<L>((float *)t.v + at, n, v);
+    }
+    if (t.w) put<L>(t.w + at, n, p);
+    put<L>((T *)t.p + at, n, p);
 }
 
 struct ValueItem { const uint8_t *codes, *exps; float *out; int64_t n; };
@@ -178,18 +179,16 @@ __global__ __launch_bounds__(256) void k_moment_values(ValueArgs a) {
     const int k = item_of(a.first, a.count, blockIdx.x);
     const ValueItem t = a.t[k];
     const bool second = a.second[k];
-    const int64_t base = (int64_t)(blockIdx.x - a.first[k]) * kSpan;
-    for (int u = 0; u < kSpan / 1024; u++) {
-        const int64_t at = base + u * 1024 + threadIdx.x * 4;
-        if (at >= t.n) return;
-        const int n = (int)(t.n - at < 4 ? t.n - at : 4), e = (int)t.exps[at / kBlock] - 127;
-        int c[4];
-        float v[4];
-        get4(t.codes + at, n, c);
+    constexpr int L = lane_values(8);
+    const int64_t at = (int64_t)(blockIdx.x - a.first[k]) * span(8) + threadIdx.x * L;
+    if (at >= t.n) return;
+    const int n = (int)(t.n - at < L ? t.n - at : L), e = (int)t.exps[at / kBlock] - 127;
+    int c[L];
+    float v[L];
+    get<L>(t.codes + at, n, c);
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = second ? decode8<true>(c[i], e) : decode8<false>(c[i], e);
-        put4(t.out + at, n, v);
-    }
+    for (int i = 0; i < L; i++) v[i] = second ? decode8<true>(c[i], e) : decode8<false>(c[i], e);
+    put<L>(t.out + at, n, v);
 }
 
 __global__ void k_adamw_tick(int64_t *step, const float *lr_dev, double lr, double b1, double b2, double wd, float *factors) {
@@ -251,7 +250,7 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
         int64_t blocks = 0;
         a.count = 0;
         for (; i < count && a.count < kItems; i++) {
-            const int64_t n = tensors[7 * (int64_t)count + i], more = (n + kSpan - 1) / kSpan;
+            const int64_t n = tensors[7 * (int64_t)count + i], more = (n + span(state_bits) - 1) / span(state_bits);
             if (n == 0) continue;
             if (a.count && blocks + more > INT32_MAX) break;
             auto at = [&](int f) { return (void *)(uintptr_t)tensors[f * (int64_t)count + i]; };
@@ -299,7 +298,7 @@ extern "C" int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_s
         a.count = 0;
         for (; i < count && a.count < 2 * kItems; i++) {
             auto at = [&](int f) { return tensors[f * (int64_t)count + i]; };
-            const int64_t n = at(3), more = (n + kSpan - 1) / kSpan;
+            const int64_t n = at(3), more = (n + span(8) - 1) / span(8);
             if (n == 0) continue;
             if (a.count && blocks + more > INT32_MAX) break;
             a.t[a.count] = ValueItem{(const uint8_t *)(uintptr_t)at(0), (const uint8_t *)(uintptr_t)at(1), (float *)(uintptr_t)at(2), n};
