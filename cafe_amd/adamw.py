@@ -25,18 +25,29 @@ class Moment8(NamedTuple):
                    torch.ones(-(-n // BLOCK), dtype=torch.uint8, device=device))
 
 
-def _check_moment8(m, n, device, what):
-    if not isinstance(m, Moment8):
-        raise ValueError(f"{what}: Moment8 expected beside Moment8, not {type(m).__name__}")
-    c, e = m
-    if (c.dtype is not torch.uint8 or e.dtype is not torch.uint8 or c.numel() != n or e.numel() != -(-n // BLOCK)
-            or c.device != device or e.device != device or not c.is_contiguous() or not e.is_contiguous()):
-        raise ValueError(f"{what}: {n} uint8 codes and {-(-n // BLOCK)} uint8 exponents, contiguous, on {device} expected")
+def _blocks(n):
+    return (n + BLOCK - 1) // BLOCK
 
 
-def _check_float(t, shape, device, what):
-    if t.dtype is not torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous float32 {tuple(shape)} on {device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _check(tensors, dtype, index, sizes, what):
+    """Every tensor of `dtype` on device `index`, contiguous, of the sizes listed (shapes, or numbers of values)."""
+    by_shape = sizes and not isinstance(sizes[0], int)
+    if not (all([t.dtype is dtype and t.get_device() == index and t.is_contiguous() for t in tensors])
+            and [t.shape if by_shape else t.numel() for t in tensors] == sizes):
+        for i, (t, n) in enumerate(zip(tensors, sizes)):
+            if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous() or (t.shape if by_shape else t.numel()) != n:
+                raise ValueError(f"{what}[{i}]: contiguous {dtype} of {n if by_shape else f'{n} values'} on the parameters' device "
+                                 f"expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_moments8(moments, counts, index, what):
+    """Moment8 throughout, codes and exponents of the right sizes; returns the lists of both."""
+    if not all([type(m) is Moment8 for m in moments]):
+        raise ValueError(f"{what}: Moment8 expected beside Moment8")
+    codes, exponents = [m[0] for m in moments], [m[1] for m in moments]
+    _check(codes, torch.uint8, index, counts, f"{what} codes")
+    _check(exponents, torch.uint8, index, [_blocks(n) for n in counts], f"{what} exponents")
+    return codes, exponents
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
@@ -57,44 +68,30 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     if n == 0:
         return
     first = params[0]
-    dtype, device = first.dtype, first.device
+    dtype, index = first.dtype, first.get_device()
     if dtype not in DTYPE_CODE:
         raise ValueError(f"float32, bfloat16 or float16 parameters expected, not {dtype}")
     eight = isinstance(exp_avgs[0], Moment8)
-    cols = [[], [], [], [], [0] * n, [0] * n, [0] * n, []]
+    shapes, counts = [p.shape for p in params], [p.numel() for p in params]
+    _check(params, dtype, index, counts, "params")
+    if not all([g.layout is torch.strided for g in grads]):
+        raise ValueError("grads: dense tensors expected")
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]             # copies live until the launch is queued
+    _check(grads, dtype, index, shapes, "grads")
+    zeros = [0] * n
+    cols = [[p.data_ptr() for p in params], [g.data_ptr() for g in grads]]
     if eight:
-        cols[4], cols[5] = [], []
-    held = []
-    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
-        if p.dtype is not dtype or p.device != device or not p.is_contiguous():
-            raise ValueError(f"params[{i}]: contiguous {dtype} on {device} expected, got {p.dtype} on {p.device}")
-        if g.dtype is not dtype or g.shape != p.shape or g.device != device or g.layout is not torch.strided:
-            raise ValueError(f"grads[{i}]: dense {dtype} {tuple(p.shape)} on {device} expected, got {g.dtype} {tuple(g.shape)} on {g.device}")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            held.append(g)
-        count = p.numel()
-        if eight:
-            _check_moment8(m, count, device, f"exp_avgs[{i}]")
-            _check_moment8(v, count, device, f"exp_avg_sqs[{i}]")
-            cols[2].append(m.codes.data_ptr())
-            cols[3].append(v.codes.data_ptr())
-            cols[4].append(m.exponents.data_ptr())
-            cols[5].append(v.exponents.data_ptr())
-        else:
-            if isinstance(m, Moment8) or isinstance(v, Moment8):
-                raise ValueError(f"moments of tensor {i}: float32 tensors expected beside float32 tensors")
-            _check_float(m, p.shape, device, f"exp_avgs[{i}]")
-            _check_float(v, p.shape, device, f"exp_avg_sqs[{i}]")
-            cols[2].append(m.data_ptr())
-            cols[3].append(v.data_ptr())
-        cols[0].append(p.data_ptr())
-        cols[1].append(g.data_ptr())
-        cols[7].append(count)
+        m8, v8 = _check_moments8(exp_avgs, counts, index, "exp_avgs"), _check_moments8(exp_avg_sqs, counts, index, "exp_avg_sqs")
+        cols += [[t.data_ptr() for t in ts] for ts in (m8[0], v8[0], m8[1], v8[1])]
+    else:
+        if any([isinstance(m, Moment8) for m in (*exp_avgs, *exp_avg_sqs)]):
+            raise ValueError("float32 moments expected beside float32 moments")
+        _check(exp_avgs, torch.float32, index, shapes, "exp_avgs")
+        _check(exp_avg_sqs, torch.float32, index, shapes, "exp_avg_sqs")
+        cols += [[t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs], zeros, zeros]
     if masters is not None:
-        for i, (p, w) in enumerate(zip(params, masters)):
-            _check_float(w, p.shape, device, f"masters[{i}]")
-        cols[6] = [w.data_ptr() for w in masters]
+        _check(masters, torch.float32, index, shapes, "masters")
+    cols += [zeros if masters is None else [w.data_ptr() for w in masters], counts]
     used = [a for a, c in zip(cols[0], cols[7]) if c]
     if len(set(used)) != len(used):
         raise ValueError("a parameter is listed twice")
@@ -106,7 +103,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
             raise _lib.CafeError("a captured step would repeat the same step number: use adamw_tick and `factors`")
         step = int(step)
     else:
-        _check_float(factors, torch.Size((3,)), device, "factors")
+        _check([factors], torch.float32, index, [3], "factors")
         step = 0
     flat = (ctypes.c_int64 * (8 * n))(*[a for c in cols for a in c])
     with launch_on(first) as st:
@@ -120,7 +117,7 @@ def adamw_tick(step, factors, *, lr, betas=(0.9, 0.999), weight_decay=0.01):
     number, or a float32 tensor of one on the same device that is read when the launch runs.  May be captured."""
     if step.dtype is not torch.int64 or step.numel() != 1 or factors.device != step.device:
         raise ValueError("step: an int64 tensor of one element, on the device of `factors`")
-    _check_float(factors, torch.Size((3,)), step.device, "factors")
+    _check([factors], torch.float32, step.get_device(), [3], "factors")
     ptr = None
     if isinstance(lr, torch.Tensor):
         if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.device != step.device:
@@ -134,22 +131,23 @@ def adamw_tick(step, factors, *, lr, betas=(0.9, 0.999), weight_decay=0.01):
 
 def moment8_values(exp_avgs, exp_avg_sqs):
     """The float32 values (1-d tensors) that two lists of Moment8 stand for, first moments and second moments, in one launch."""
-    both = [(m, 0) for m in exp_avgs] + [(v, 1) for v in exp_avg_sqs]
+    both = [*exp_avgs, *exp_avg_sqs]
     if not both:
         return [], []
-    device = both[0][0].codes.device
-    cols, out = [[], [], [], [], []], []
-    for m, second in both:
-        n = m.codes.numel()
-        _check_moment8(m, n, device, "moment")
-        out.append(torch.empty(n, dtype=torch.float32, device=device))
-        for c, a in zip(cols, (m.codes.data_ptr(), m.exponents.data_ptr(), out[-1].data_ptr(), n, second)):
-            c.append(a)
-    on_device(both[0][0].codes)
-    flat = (ctypes.c_int64 * (5 * len(both)))(*[a for c in cols for a in c])
-    with launch_on(both[0][0].codes) as st:
-        _lib.check(_lib.load().cafe_moment8_values_dev(flat, len(both), st), "cafe_moment8_values_dev")
-    return out[:len(exp_avgs)], out[len(exp_avgs):]
+    if not isinstance(both[0], Moment8):
+        raise ValueError(f"Moment8 expected, not {type(both[0]).__name__}")
+    first = both[0].codes
+    counts = [m[0].numel() for m in both]
+    codes, exponents = _check_moments8(both, counts, first.get_device(), "moments")
+    on_device(first)
+    sizes = [v for n in counts for v in (n, -n & 3)]             # slices of one array, on boundaries of 16 bytes
+    out = torch.empty(sum(sizes), dtype=torch.float32, device=first.device).split(sizes)[::2]
+    cols = ([t.data_ptr() for t in codes], [t.data_ptr() for t in exponents], [t.data_ptr() for t in out], counts,
+            [0] * len(exp_avgs) + [1] * len(exp_avg_sqs))
+    table = (ctypes.c_int64 * (5 * len(both)))(*[a for c in cols for a in c])
+    with launch_on(first) as st:
+        _lib.check(_lib.load().cafe_moment8_values_dev(table, len(both), st), "cafe_moment8_values_dev")
+    return list(out[:len(exp_avgs)]), list(out[len(exp_avgs):])
 
 
 class AdamW(torch.optim.Optimizer):
