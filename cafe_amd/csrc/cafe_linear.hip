@@ -11,7 +11,6 @@
 #include "cafe_dense.h"
 
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <cmath>
@@ -268,15 +267,15 @@ template <int MF, int R, int W, int V> __device__ __forceinline__ void weave() {
     weave_all<MF, R, W, V>(std::make_integer_sequence<int, R + W + V>{});
 }
 
-// C tile of BM x BN by four waves in 2 x 2, each (BM / 2) x (BN / 2) in 32 x 32 MFMA blocks.  Two LDS buffers, one barrier
-// per 128 bytes of reduction: a wave that writes buffer k % 2 has passed the barrier behind every read of it.  PF tiles
-// are on their way in registers: a float32 tile computes for longer than memory takes to answer (64 products of 64
-// cycles per wave), a 16-bit one (16 of 32) does not.
-template <class T, bool ACOLS, bool BCOLS, int BM, int BN>
-__global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
-    constexpr int TI = BM / 64, TJ = BN / 64, E = Elem<T>::per_chunk, PF = sizeof(T) == 4 ? 1 : 2;
-    typedef Operand<T, ACOLS, BM, 256> OA;
-    typedef Operand<T, BCOLS, BN, 256> OB;
+// C tile of BM x BN by WM x WN waves, each (BM / WM) x (BN / WN) in 32 x 32 MFMA blocks.  Two LDS buffers, one barrier per
+// 128 bytes of reduction: a wave that writes buffer k % 2 has passed the barrier behind every read of it.  PF tiles are on
+// their way in registers: a float32 tile computes for longer than memory takes to answer (64 products of 64 cycles per
+// wave), a 16-bit one (16 of 32) does not.
+template <class T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
+    constexpr int TH = WM * WN * 64, TI = BM / WM / 32, TJ = BN / WN / 32, E = Elem<T>::per_chunk, PF = sizeof(T) == 4 ? 1 : 2;
+    typedef Operand<T, ACOLS, BM, TH> OA;
+    typedef Operand<T, BCOLS, BN, TH> OB;
     constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, CS = BN + 8;
     __shared__ __align__(16) char lds[2 * STAGE > BM * CS * 4 ? 2 * STAGE : BM * CS * 4];
     const int tile = xcd_tile(blockIdx.x, g.tiles);
@@ -284,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
     const int64_t kts = (g.R + BK - 1) / BK;
     const int64_t k0 = kts * blockIdx.y / g.slices, k1 = kts * (blockIdx.y + 1) / g.slices;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int wi = (wave >> 1) * (BM / 2), wj = (wave & 1) * (BN / 2);
+    const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
     f32x16 acc[TI][TJ];
 #pragma unroll
     for (int a = 0; a < TI; a++)
@@ -401,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
     // The tile goes through LDS, so that a thread ends up with neighbouring columns of a row: 16-byte accesses to
     // everything that follows.  Accumulator element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
     float *c = (float *)lds;
-    if (sums) {                                 // 256 / CPR threads hold partial sums of the same columns
+    if (sums) {                                 // TH / CPR threads hold partial sums of the same columns
         for (int e = 0; e < E; e++) c[threadIdx.x * E + e] = cs[e];
         __syncthreads();
         if (threadIdx.x < BM && i0 + threadIdx.x < g.I) {
@@ -421,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
             for (int e = 0; e < 16; e++)
                 c[(wi + 32 * a + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * CS + wj + 32 * b + (lane & 31)] = acc[a][b][e];
     __syncthreads();
-    constexpr int CH = BN / E, PASS = BM * CH / 256;
+    constexpr int CH = BN / E, PASS = BM * CH / TH;
     const int col = threadIdx.x % CH * E;
     const int64_t j = j0 + col;
     const int left = (int)(g.J - j < E ? g.J - j : E);
@@ -430,7 +429,7 @@ __global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
         float *part = g.o.part + (int64_t)blockIdx.y * g.I * g.J;
 #pragma unroll 2
         for (int q = 0; q < PASS; q++) {
-            const int row = threadIdx.x / CH + q * (256 / CH);
+            const int row = threadIdx.x / CH + q * (TH / CH);
             const int64_t i = i0 + row;
             if (i >= g.I) break;
 #pragma unroll
@@ -443,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void k_tile(TileArgs g) {
     auto put = [&](auto actc) {
 #pragma unroll 2
         for (int q = 0; q < PASS; q++) {
-            const int row = threadIdx.x / CH + q * (256 / CH);
+            const int row = threadIdx.x / CH + q * (TH / CH);
             const int64_t i = i0 + row;
             if (i >= g.I) break;
             float v[E];
@@ -628,48 +627,52 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 //     steps x max(alone, load x shared) + load x ends + join
 //
 // steps: 128-byte steps of the reduction per slice; load: workgroups per compute unit; shared, alone: what a step costs
-// a compute unit among workgroups that fill it and in one that runs by itself (128 x 128, one side 64, 64 x 64); ends:
-// loading the first tile and storing the result; join: the second launch, the way of the partial sums out and back
-// (2.5 TB/s) and the slices.  The constants are fitted to 1500 timings of 45 products between 1 x 256 x 8192 and 16384 x
-// 3341 x 256 in float32 and bfloat16; the choice is within 1.2 % of the fastest on average and 27 % off at worst (1 x 256
-// outputs over 8192 in bfloat16).  Both sides of it: 8192 x 256 outputs over 512 in bfloat16 take 8.0 us in 64 x 64 tiles
-// and 10.5 in 128 x 128 (half the units idle), 8192 x 1024 over 1024 take 30.8 and 25.0; 64 x 256 outputs over 8192 in
-// float32 take 14.7 us in 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and 11.9 in 12.
+// a compute unit among workgroups that fill it and in one that runs by itself (256 x 128 for 16-bit types, 128 x 128, one
+// side 64, 64 x 64); ends: loading the first tile and storing the result; join: the second launch, the way of the partial sums
+// out and back (2.5 TB/s) and the slices.  The constants are fitted to 1700 timings of 45 products between 1 x 256 x 8192
+// and 16384 x 3341 x 256 in float32 and bfloat16; the choice is within 1.2 % of the fastest on average and 25 % off at
+// worst (1 x 256 outputs over 8192 in bfloat16).  Both sides of it, bfloat16: 8192 x 256 outputs over 512 take 8.0 us in
+// 64 x 64 tiles, 10.5 in 128 x 128 (half the units idle), 12.6 in 256 x 128; 8192 x 1024 over 1024 (dx) take 34.8, 28.2 and
+// 24.7; in float32 256 x 128 gains 2 % there and loses 5 % in slices.  float32: 64 x 256 outputs over 8192 take 14.7 us in 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and
+// 11.9 in 12.
 struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; double us; };
-struct Cost { double shared[3], alone[3], ends, join, per_slice, launch; };
+struct Cost { double shared[4], alone[4], ends, join, per_slice, launch; };
 
 Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
-    static const Cost f32 = {{1.82, 1.0, 0.535}, {2.32, 1.18, 0.65}, 2.5, 1.7, 0.065, 4.7};
-    static const Cost half = {{0.585, 0.43, 0.28}, {0.80, 0.56, 0.31}, 1.7, 2.3, 0.14, 4.4};
+    static const Cost f32 = {{0, 1.85, 1.01, 0.54}, {0, 2.25, 1.25, 0.68}, 2.4, 1.8, 0.05, 4.8};
+    static const Cost half = {{0.94, 0.6, 0.41, 0.28}, {0.94, 0.785, 0.56, 0.315}, 1.4, 2.2, 0.14, 4.6};
+    static const struct { int bm, bn, kind; } tiles[] = {{256, 128, 0}, {128, 128, 1}, {128, 64, 2}, {64, 128, 2}, {64, 64, 3}};
     const Cost &c = dtype == kF32 ? f32 : half;
     const int64_t bk = 128 / elem_size(dtype), kts = (R + bk - 1) / bk;
     Plan best = {};
-    double least = 0;
-    for (int bm = 128; bm >= 64; bm /= 2)
-        for (int bn = 128; bn >= 64; bn /= 2) {
-            const int kind = (bm == 64) + (bn == 64);
-            const int64_t ti = (I + bm - 1) / bm, tj = std::max<int64_t>(1, (J + bn - 1) / bn);
-            for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64}) {
-                if (s > 1 && (ti * tj * s > 2048 || kts < 2 * s)) break;
-                const double load = std::ceil((double)ti * tj * s / 256.0), steps = (double)((kts + s - 1) / s);
-                double t = steps * std::max(c.alone[kind], c.shared[kind] * load) + c.ends * load * (bm * bn) / 16384.0;
-                if (s > 1) t += c.join + c.per_slice * s + 4e-7 * 4 * s * (double)I * J;
-                if (best.bm == 0 || t < least) { least = t; best = Plan{bm, bn, ti, tj, ti * tj, s, 0, t + c.launch}; }
-            }
+    for (const auto &t : tiles) {
+        if (t.kind == 0 && dtype == kF32) continue;
+        const int64_t ti = (I + t.bm - 1) / t.bm, tj = std::max<int64_t>(1, (J + t.bn - 1) / t.bn);
+        for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64}) {
+            if (s > 1 && (ti * tj * s > 2048 || kts < 2 * s)) break;
+            const double load = std::ceil((double)ti * tj * s / 256.0), steps = (double)((kts + s - 1) / s);
+            double us = c.launch + steps * std::max(c.alone[t.kind], c.shared[t.kind] * load) + c.ends * load * (t.bm * t.bn) / 16384.0;
+            if (s > 1) us += c.join + c.per_slice * s + 4e-7 * 4 * s * (double)I * J;
+            if (best.bm == 0 || us < best.us) best = Plan{t.bm, t.bn, ti, tj, ti * tj, s, 0, us};
         }
-#ifdef CAFE_TUNE
-    if (const char *e = getenv("CAFE_TUNE_PLAN")) { sscanf(e, "%d,%d,%d", &best.bm, &best.bn, &best.slices); best.tiles_i=(I+best.bm-1)/best.bm; best.tiles_j=std::max<int64_t>(1,(J+best.bn-1)/best.bn); best.tiles=best.tiles_i*best.tiles_j; }
-#endif
+    }
     best.ws = best.slices > 1 ? up256((int64_t)best.slices * I * J * 4) : 0;
     return best;
 }
 
 template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, hipStream_t st) {
     const dim3 grid((unsigned)g.tiles, (unsigned)p.slices);
-    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128>), grid, dim3(256), 0, st, g);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64>), grid, dim3(256), 0, st, g);
-    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64>), grid, dim3(256), 0, st, g);
+    if constexpr (sizeof(T) == 2) {
+        if (p.bm == 256) {
+            hipLaunchKernelGGL((k_tile<T, AC, BC, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
+            CAFE_HIP_CHECK(hipGetLastError());
+            return 0;
+        }
+    }
+    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
 }
