@@ -464,18 +464,31 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
     }
 }
 
-// Sum of the reduction's slices in their order, then what follows the product; the blocks behind `out_blocks` join the
-// column sums.
+// Sum of the reduction's slices in their order, then what follows the product; the blocks behind `out_blocks` join
+// `parts` rows of column sums, 16 columns in 16 runs of rows at a time.
 template <class T, int ACT>
-__global__ __launch_bounds__(256) void k_join(Out o, int64_t I, int64_t J, int slices, int out_blocks, const float *sums, T *sums_out) {
+__global__ __launch_bounds__(256) void k_join(Out o, int64_t I, int64_t J, int slices, int out_blocks, const float *sums, int parts, T *sums_out) {
     constexpr int E = Elem<T>::per_chunk;
     if ((int)blockIdx.x >= out_blocks) {
-        const int64_t i = (int64_t)(blockIdx.x - out_blocks) * 256 + threadIdx.x;
-        if (i >= I) return;
-        float v = 0.f;
+        __shared__ float run[16][16];
+        const int x = threadIdx.x & 15, y = threadIdx.x >> 4;
+        for (int64_t i0 = (int64_t)(blockIdx.x - out_blocks) * 16; i0 < I; i0 += (int64_t)(gridDim.x - out_blocks) * 16) {
+            const int64_t i = i0 + x;
+            float v = 0.f;
+            if (i < I) {
 #pragma unroll 8
-        for (int s = 0; s < slices; s++) v += sums[s * I + i];
-        sums_out[i] = (T)v;
+                for (int s = parts * y / 16; s < parts * (y + 1) / 16; s++) v += sums[s * I + i];
+            }
+            run[y][x] = v;
+            __syncthreads();
+            if (y == 0 && i < I) {
+                v = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; r++) v += run[r][x];
+                sums_out[i] = (T)v;
+            }
+            __syncthreads();
+        }
         return;
     }
     const int64_t chunks = (J + E - 1) / E, n = I * chunks;
@@ -529,7 +542,8 @@ template <class T, int FT, int WAVES, bool MANY_W> __global__ __launch_bounds__(
     __shared__ float part[WAVES][FT * 4][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int64_t many = MANY_W ? g.N : g.M, few = MANY_W ? g.M : g.N, K = g.K;
-    const int64_t i0 = (int64_t)blockIdx.x * 16;
+    const int64_t i0 = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16;
+    if (i0 >= many) return;
     const T *pa = (const T *)g.many + (i0 + r < many ? i0 + r : many - 1) * g.ldm + q * E;
     const T *pb[FT];
 #pragma unroll
@@ -594,25 +608,61 @@ template <class T, int FT, int WAVES, bool MANY_W> __global__ __launch_bounds__(
 }
 
 // dz = dy * act'(z), rounded.  kept: z in the type (relu: anything of its sign), or the slopes in float32.  One 16-byte
-// chunk per thread and step.
+// chunk per thread and step.  SUMS: the column sums of the unrounded values over the block's rows, a row of `sums` per
+// blockIdx.y; a block then has `lanes` chunks side by side.
+template <class T, int ACT> __device__ __forceinline__ void dz_chunk(const T *dy, const void *kept, int64_t at_kept, T *dz, int left, float *g) {
+    constexpr int E = Elem<T>::per_chunk;
+    float k[E];
+    unpack<T>(load_some(dy, left), g);
+    if constexpr (ACT == ACT_SLOPE) {
+#pragma unroll
+        for (int h = 0; h < E; h += 4) unpack<float>(load_some((const float *)kept + at_kept + h, left - h), k + h);
+    } else {
+        unpack<T>(load_some((const T *)kept + at_kept, left), k);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) g[e] = through<ACT>(g[e], k[e]);
+    store_some(dz, pack<T>(g), left);
+}
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t M, int64_t N) {
     constexpr int E = Elem<T>::per_chunk;
     const int64_t chunks = (N + E - 1) / E, n = M * chunks;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
         const int64_t m = q / chunks, col = (q - m * chunks) * E;
-        const int left = (int)(N - col < E ? N - col : E);
-        float g[E], k[E];
-        unpack<T>(load_some(dy + m * ldy + col, left), g);
-        if constexpr (ACT == ACT_SLOPE) {
+        float g[E];
+        dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, (int)(N - col < E ? N - col : E), g);
+    }
+}
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t M, int64_t N,
+                                                int lanes, int64_t rows, float *sums) {
+    constexpr int E = Elem<T>::per_chunk;
+    __shared__ float red[256 * E];
+    const int x = threadIdx.x % lanes, y = threadIdx.x / lanes, ny = 256 / lanes;
+    const int64_t col = ((int64_t)blockIdx.x * lanes + x) * E, m1 = (blockIdx.y + 1) * rows < M ? (blockIdx.y + 1) * rows : M;
+    const int left = (int)(N - col < E ? N - col : E);
+    float s[E];
 #pragma unroll
-            for (int h = 0; h < E; h += 4) unpack<float>(load_some((const float *)kept + m * ldk + col + h, left - h), k + h);
-        } else {
-            unpack<T>(load_some((const T *)kept + m * ldk + col, left), k);
+    for (int e = 0; e < E; e++) s[e] = 0.f;
+    if (left > 0) {
+#pragma unroll 4
+        for (int64_t m = blockIdx.y * rows + y; m < m1; m += ny) {
+            float g[E];
+            dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, left, g);
+#pragma unroll
+            for (int e = 0; e < E; e++) s[e] += g[e];
         }
+    }
 #pragma unroll
-        for (int e = 0; e < E; e++) g[e] = through<ACT>(g[e], k[e]);
-        store_some(dz + m * N + col, pack<T>(g), left);
+    for (int e = 0; e < E; e++) red[threadIdx.x * E + e] = s[e];
+    __syncthreads();
+    for (int w = threadIdx.x; w < lanes * E; w += 256) {
+        const int64_t c = (int64_t)blockIdx.x * lanes * E + w;
+        if (c >= N) continue;
+        float v = 0.f;
+        for (int r = 0; r < ny; r++) v += red[r * lanes * E + w];
+        sums[blockIdx.y * N + c] = v;
     }
 }
 
@@ -633,8 +683,8 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 // and 16384 x 3341 x 256 in float32 and bfloat16; the choice is within 1.2 % of the fastest on average and 25 % off at
 // worst (1 x 256 outputs over 8192 in bfloat16).  Both sides of it, bfloat16: 8192 x 256 outputs over 512 take 8.0 us in
 // 64 x 64 tiles, 10.5 in 128 x 128 (half the units idle), 12.6 in 256 x 128; 8192 x 1024 over 1024 (dx) take 34.8, 28.2 and
-// 24.7; in float32 256 x 128 gains 2 % there and loses 5 % in slices.  float32: 64 x 256 outputs over 8192 take 14.7 us in 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and
-// 11.9 in 12.
+// 24.7; in float32 256 x 128 gains 2 % there and loses 5 % in slices.  float32: 64 x 256 outputs over 8192 take 14.7 us in
+// 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and 11.9 in 12.
 struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; double us; };
 struct Cost { double shared[4], alone[4], ends, join, per_slice, launch; };
 
@@ -661,6 +711,10 @@ Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
 }
 
 template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, hipStream_t st) {
+    if (p.tiles > (int64_t)1 << 22) {                       // a grid holds fewer than 2^32 work items; INT32_MAX tiles are far behind it
+        set_error("cafe_linear: %lld tiles of %d x %d are more than a launch takes", (long long)p.tiles, p.bm, p.bn);
+        return 1;
+    }
     const dim3 grid((unsigned)g.tiles, (unsigned)p.slices);
     if constexpr (sizeof(T) == 2) {
         if (p.bm == 256) {
@@ -688,46 +742,65 @@ template <class F> void with_act(int act, F f) {
     }
 }
 
-// C = A B^T (+ what follows) for operands of type T; `part`, `sums`: workspace of p.ws and p.sums_ws bytes.  sums_out: the
-// sums of A's columns (gradient of a bias), or null.  g.o.y == null: the sums alone.
-template <class T, bool AC, bool BC> int product(const Plan &p, TileArgs g, float *part, float *sums, T *sums_out, hipStream_t st) {
+// Joins a product's slices and `parts` rows of column sums (either may be missing).
+template <class T> int join(const Plan &p, const TileArgs &g, const Out &o, float *part, const float *sums, int parts, T *sums_out, hipStream_t st) {
+    constexpr int E = Elem<T>::per_chunk;
+    Out j = o;
+    j.part = part;
+    const int out_blocks = part ? (int)std::min<int64_t>((g.I * ((g.J + E - 1) / E) + 255) / 256, 256 * 16) : 0;
+    const int sum_blocks = sums_out ? (int)std::min<int64_t>((g.I + 15) / 16, 1 << 16) : 0;
+    with_act(o.act, [&](auto a) {
+        hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3((unsigned)(out_blocks + sum_blocks)), dim3(256), 0, st, j, g.I, g.J, p.slices,
+                           out_blocks, sums, parts, sums_out);
+    });
+    CAFE_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+// C = A B^T (+ what follows) for operands of type T; `part`, `sums`: workspace.  sums_out: the sums of A's columns (gradient
+// of a bias), or null; they are formed here, or were left in `parts` rows of `sums`.  g.o.y == null: the sums alone.
+template <class T, bool AC, bool BC>
+int product(const Plan &p, TileArgs g, float *part, float *sums, int parts, T *sums_out, hipStream_t st) {
     if (g.I == 0 || (g.J == 0 && !sums_out)) return 0;
     const bool out = g.o.y != nullptr && g.J > 0;
+    if (!out && parts) return join<T>(p, g, g.o, nullptr, sums, parts, sums_out, st);
     if (!out) { g.b = g.a; g.ldb = g.lda; g.J = g.I; g.o.y = nullptr; }      // one column of tiles, whose products nobody reads
     const Out o = g.o;
     g.tiles_j = out ? (int)p.tiles_j : 1;
     g.tiles = (int)p.tiles_i * g.tiles_j;
     g.slices = p.slices;
-    g.sums = sums_out ? sums : nullptr;
+    g.sums = sums_out && !parts ? sums : nullptr;
     g.sums_out = p.slices == 1 ? sums_out : nullptr;
     if (p.slices > 1 && out) g.o.part = part;
     if (launch_tile<T, AC, BC>(p, g, st)) return 1;
-    if (p.slices > 1) {
-        Out j = o;
-        j.part = part;
-        constexpr int E = Elem<T>::per_chunk;
-        const int out_blocks = out ? (int)std::min<int64_t>((g.I * ((g.J + E - 1) / E) + 255) / 256, 256 * 16) : 0;
-        const int sum_blocks = sums_out ? (int)((g.I + 255) / 256) : 0;
-        with_act(o.act, [&](auto a) {
-            hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3((unsigned)(out_blocks + sum_blocks)), dim3(256), 0, st, j, g.I, g.J, p.slices,
-                               out_blocks, sums, sums_out);
-        });
-        CAFE_HIP_CHECK(hipGetLastError());
-    }
-    return 0;
+    if (p.slices == 1 && !parts) return 0;
+    return join<T>(p, g, o, p.slices > 1 && out ? part : nullptr, sums, parts ? parts : p.slices, sums_out, st);
 }
 
 // dz is formed once, rounded to the type, ahead of both products.  Formed in their loads instead (dy times the slopes, two
 // operands read in place of one) it cost float32 more than it saved: 321 us against 307 at 8192 x 1024 x 1024; 16-bit
-// types would read both once per column of tiles.
+// types would read both once per column of tiles.  Where dz is rounded, the pass that forms it adds up the bias gradient
+// from the unrounded values; elsewhere dW's tiles add up the columns they read anyway.
+struct DzPlan { int lanes, parts; int64_t blocks_x, rows; };
+DzPlan dz_plan(int64_t M, int64_t N, int dtype, int act) {
+    DzPlan d = {};
+    if (dtype == kF32 || act == ACT_NONE || act == ACT_RELU || M == 0 || N == 0) return d;
+    const int64_t chunks = (N + 7) / 8;
+    for (d.lanes = 1; d.lanes < 64 && d.lanes < chunks;) d.lanes *= 2;
+    d.blocks_x = (chunks + d.lanes - 1) / d.lanes;
+    const int64_t ny = 256 / d.lanes, want = std::max<int64_t>(1, std::min<int64_t>(256, 2048 / d.blocks_x));
+    d.rows = std::max<int64_t>(ny, (M + want - 1) / want);
+    d.parts = (int)((M + d.rows - 1) / d.rows);
+    return d;
+}
 
-// workspace of the backward: [dz][column sums of the slices][partial products, used by dx, then by dW]
+// workspace of the backward: [dz][column sums of the slices or of dz's blocks][partial products, used by dx, then by dW]
 struct BwdWs { int64_t sums, part, bytes; };
 BwdWs bwd_ws(int64_t M, int64_t K, int64_t N, int dtype, int act) {
     BwdWs w;
     const Plan dx = plan(M, K, N, dtype), dw = plan(N, K, M, dtype);
     w.sums = act == ACT_NONE ? 0 : up256(M * N * elem_size(dtype));
-    w.part = w.sums + up256((int64_t)dw.slices * N * 4);
+    w.part = w.sums + up256((int64_t)std::max(dw.slices, dz_plan(M, N, dtype, act).parts) * N * 4);
     w.bytes = w.part + std::max(dx.ws, dw.ws);
     return w;
 }
@@ -745,9 +818,10 @@ bool bad_sizes(const char *who, int64_t m, int64_t k, int64_t n, int dtype, int 
 
 template <class T, int FT, bool MANY_W> int launch_skinny(const SkinnyArgs &g, hipStream_t st) {
     const int64_t many = MANY_W ? g.N : g.M;
-    const unsigned blocks = (unsigned)((many + 15) / 16);
-    if (many <= 16 * 512) hipLaunchKernelGGL((k_skinny<T, FT, 8, MANY_W>), dim3(blocks), dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((k_skinny<T, FT, 4, MANY_W>), dim3(blocks), dim3(256), 0, st, g);
+    const int64_t blocks = (many + 15) / 16, wide = 1 << 20;
+    const dim3 grid((unsigned)std::min(blocks, wide), (unsigned)((blocks + wide - 1) / wide));
+    if (many <= 16 * 512) hipLaunchKernelGGL((k_skinny<T, FT, 8, MANY_W>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_skinny<T, FT, 4, MANY_W>), grid, dim3(256), 0, st, g);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -775,7 +849,7 @@ template <class T> int fwd(TileArgs g, void *ws, int dtype, hipStream_t st) {
         if (g.I <= g.J) return skinny<T, true>(SkinnyArgs{g.b, g.a, g.ldb, g.lda, g.I, g.J, g.R, g.o}, st);
         return skinny<T, false>(SkinnyArgs{g.a, g.b, g.lda, g.ldb, g.I, g.J, g.R, g.o}, st);
     }
-    return product<T, false, false>(plan(g.I, g.J, g.R, dtype), g, (float *)ws, nullptr, nullptr, st);
+    return product<T, false, false>(plan(g.I, g.J, g.R, dtype), g, (float *)ws, nullptr, 0, nullptr, st);
 }
 int64_t fwd_ws(int64_t m, int64_t k, int64_t n, int dtype) {
     return is_skinny(m, k, n, dtype, dtype == kF32) ? 0 : plan(m, n, k, dtype).ws;      // whatever the alignment turns out to be
@@ -788,11 +862,17 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
     float *sums = (float *)(ws + at.sums), *part = (float *)(ws + at.part);
     const T *dz = dy;
     int64_t lddz = lddy;
+    DzPlan d = {};
     if (act != ACT_NONE && M > 0 && N > 0 && (dx || dw || db)) {
         T *z = (T *)ws;
         constexpr int E = Elem<T>::per_chunk;
         const unsigned blocks = (unsigned)std::min<int64_t>((M * ((N + E - 1) / E) + 255) / 256, 256 * 32);
-        with_act(act, [&](auto a) { hipLaunchKernelGGL((k_dz<T, decltype(a)::value>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, M, N); });
+        if (db) d = dz_plan(M, N, dtype, act);
+        with_act(act, [&](auto a) {
+            if (d.parts) hipLaunchKernelGGL((k_dz_sums<T, decltype(a)::value>), dim3((unsigned)d.blocks_x, (unsigned)d.parts), dim3(256), 0, st, dy, lddy,
+                                            kept, ldk, z, M, N, d.lanes, d.rows, sums);
+            else hipLaunchKernelGGL((k_dz<T, decltype(a)::value>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, M, N);
+        });
         CAFE_HIP_CHECK(hipGetLastError());
         dz = z; lddz = N;
     }
@@ -802,13 +882,13 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
         TileArgs q = g;
         q.b = w; q.ldb = ldw; q.I = M; q.J = K; q.R = N;
         q.o.y = dx; q.o.ldy = lddx;
-        if (product<T, false, true>(plan(M, K, N, dtype), q, part, nullptr, nullptr, st)) return 1;
+        if (product<T, false, true>(plan(M, K, N, dtype), q, part, nullptr, 0, nullptr, st)) return 1;
     }
     if (dw || db) {
         TileArgs q = g;
         q.b = x; q.ldb = ldx; q.I = N; q.J = K; q.R = M;
         q.o.y = dw; q.o.ldy = K;
-        return product<T, true, true>(plan(N, K, M, dtype), q, part, sums, db, st);
+        return product<T, true, true>(plan(N, K, M, dtype), q, part, sums, d.parts, db, st);
     }
     return 0;
 }

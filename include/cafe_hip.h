@@ -329,9 +329,10 @@ void cafe_ae_ref_update(int idx);
 /* y[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + res[M, N], all of one type, sums in float32 (dlrm_s_pytorch.py:213-251:
  * a Linear and its activation; wdl.py:704-721: the last deep layer with the wide part's logit as `res`).
  * act: 0 none, 1 relu, 2 sigmoid, 3 gelu (z Phi(z)), 4 silu.  d_bias, d_res, d_kept may be null.  d_kept [M, N] receives
- * act'(z) in float32 (rounded to 16 bits, it would cost the gradients one more rounding than they have): what the backward
- * of sigmoid, gelu and silu needs, and relu's where `res` hides the sign of its output.  ldx, ldw and ldr may be 0 (one row repeated); ldy and ldk at least n.
- * m, n or k may be 0 (k == 0: the sum is 0).  Workspace: cafe_linear_fwd_ws bytes (-1: bad sizes). */
+ * act'(z) in float32 (rounded to 16 bits, it would cost the gradients one more rounding than they have): what the
+ * backward of sigmoid, gelu and silu needs, and relu's where `res` hides the sign of its output.  ldx, ldw and ldr may be
+ * 0 (one row repeated); ldy and ldk at least n.  m, n or k may be 0 (k == 0: the sum is 0).  Workspace:
+ * cafe_linear_fwd_ws bytes (-1: bad sizes), on a boundary of 16 bytes. */
 int64_t cafe_linear_fwd_ws(int64_t m, int64_t k, int64_t n, int dtype);
 int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, const void *d_res,
                         int64_t ldr, void *d_y, int64_t ldy, float *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
@@ -339,9 +340,9 @@ int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t l
 /* Gradients of the same: dz = dy * act'(kept); dx[M, K] = dz w, dw[N, K] = dz^T x (contiguous), db[N] = column sums of dz.
  * Any of d_dx, d_dw, d_db may be null (not wanted).  d_kept [M, N]: for act 2, 3, 4 the value before the activation; for
  * relu that or its output (only the sign is read), of type `dtype`; for act 5 the float32 slopes act'(z) of any
- * activation, as the forward wrote them; not read for act 0.  dz is rounded to the type before the products (they run on the
- * matrix units); db sums the same values.  The result does not depend on the run: every sum has a
- * fixed order. */
+ * activation, as the forward wrote them; not read for act 0.  dz is rounded to the type before the products (they run on
+ * the matrix units); db sums the unrounded values.  The result does not depend on the run: every sum has a fixed order.
+ * Workspace: cafe_linear_bwd_ws bytes (-1: bad sizes), on a boundary of 16 bytes. */
 int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype, int act);
 int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw,
                         const void *d_kept, int64_t ldk, void *d_dx, int64_t lddx, void *d_dw, void *d_db, int64_t m, int64_t k,
@@ -360,11 +361,11 @@ int cafe_interact_bwd_dev(const void *d_dout, int64_t lddo, const void *d_x, int
                           int emb_dtype, int dtype, void *d_dx, int64_t lddx, void *d_demb, int64_t dfield_stride,
                           int64_t dbatch_stride, cafe_stream_t stream);
 
-/* One AdamW step in place over `count` tensors (the dense parameters of a head; the reference steps them with torch.optim).  `tensors` is a
- * HOST array of eight columns of `count` int64 each, copied before the call returns: addresses of p, g, m, v, exponents of
+/* One AdamW step in place over `count` tensors (the dense parameters of a head; the reference steps them with
+ * torch.optim).  `tensors` is a HOST array of eight columns of `count` int64 each, copied before the call returns: addresses of p, g, m, v, exponents of
  * m, exponents of v (0 with 32-bit states), float32 master weights (0: none), number of values.  p and g are of type
  * `dtype`, any element alignment; m and v float32 (state_bits 32) or one code per value with one exponent byte per 256
- * values (state_bits 8; the format stands in cafe_adamw.hip).  No two tensors may overlap.
+ * values (state_bits 8; the format stands in cafe_adamw.hip).  No two tensors may overlap (a float32 p and its own master may).
  *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)
  * d_factors != null: {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd} are read from the device (cafe_adamw_tick_dev) and
  * lr and step are not used, so that the call can be captured and replayed. */

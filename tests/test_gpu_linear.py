@@ -85,7 +85,7 @@ def check_backward(grads, dy, x, w, kept, act):
     for got, want, err, what in (
             (dx, dz @ wd, rz @ wd.abs() + (2 * n + 16) * U32 * (dz.abs() @ wd.abs()), "dx"),
             (dw, dz.t() @ xd, rz.t() @ xd.abs() + (2 * m + 16) * U32 * (dz.t().abs() @ xd.abs()), "dw"),
-            (db, dz.sum(0), rz.sum(0) + (2 * m + 16) * U32 * dz.abs().sum(0), "db")):
+            (db, dz.sum(0), ez.sum(0) + (2 * m + 16) * U32 * dz.abs().sum(0), "db")):
         if got is not None:
             check(got, want, err + half_step(t) * 1.01 * want.abs() + tiny(t), what)
 
@@ -315,3 +315,57 @@ def test_mlp_of_modules(t):
         d, dw, db = linear_backward(d, h, w, kept, act)
         want = [dw, db] + want
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_more_rows_than_a_grid_is_wide(t):
+    """One output column: 16 rows per workgroup, 2^20 workgroups side by side, the rest in a second row of them."""
+    m, k = 16 * 2 ** 20 + 50, 5
+    x, w, b, _, _ = make(4, k, 1, t)
+    x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(t)
+    y = linear(x, w, b)
+    xd, wd = x.double(), w.double()
+    want = xd @ wd.t() + b.double()
+    check(y, want, sum_error(xd, wd, k) + 4 * U32 * want.abs() + half_step(t) * 1.01 * want.abs() + tiny(t), "y")
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_offsets_past_32_bits(t):
+    """Rows 2^24 elements apart: the last ones start behind 2^31 elements, in every operand of both passes."""
+    m, k, n, far = 150, 130, 200, 2 ** 24
+    x, w, b, _, dy = make(m, k, n, t)
+
+    def spread(a):
+        out = torch.empty((a.shape[0] - 1) * far + a.shape[1], dtype=t, device="cuda").as_strided(a.shape, (far, 1))
+        out.copy_(a)
+        return out
+    near = linear_forward(x, w, b, "silu")
+    want = linear_backward(dy, x, w, near[1], "silu")
+    xs = spread(x)
+    assert torch.equal(linear_forward(xs, w, b, "silu")[0], near[0])
+    got = linear_backward(dy, xs, w, near[1], "silu")
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    del xs
+    ws = spread(w)
+    assert torch.equal(linear_forward(x, ws, b, "silu")[0], near[0])
+    got = linear_backward(dy, x, ws, near[1], "silu")
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    del ws
+    ds = spread(dy)
+    got = linear_backward(ds, x, w, near[1], "silu")
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    del ds
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_the_bias_gradient_alone(t, act):
+    """The same bits as beside the other gradients, for one product of slices and for a whole one."""
+    for m, k, n in ((70, 30, 50), (5000, 20, 33), (3, 200, 600)):
+        x, w, b, _, dy = make(m, k, n, t)
+        kept = linear_forward(x, w, b, act)[1]
+        want = linear_backward(dy, x, w, kept, act)
+        db = linear_backward(dy, x, w, kept, act, need=(False, False, True))
+        assert db[0] is None and db[1] is None and torch.equal(db[2], want[2])
