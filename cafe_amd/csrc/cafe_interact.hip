@@ -21,7 +21,7 @@ struct InteractArgs {
     const void *dout; int64_t lddo;
     void *dx; int64_t lddx;
     void *demb; int64_t dsf, dsb;
-    int64_t B;
+    int64_t B, b0;                                  // samples b0 .. B - 1 are this launch's
     int F, D, nf, pairs, itself, lead;              // lead: D with dense features, else 0
 };
 
@@ -75,7 +75,7 @@ template <class TE, class T, int RT> __global__ __launch_bounds__(256) void k_in
     constexpr int E = Elem<TE>::per_chunk, ET = Elem<T>::per_chunk, STEP = 4 * E, U = RT <= 2 ? 4 : RT <= 4 ? 2 : 1;
     extern __shared__ float lds[];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t b = g.b0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (b >= g.B) return;
     const bool isx = g.lead && r == 0;                  // row 0 of tile 0
     const T *px = (const T *)g.x + b * g.ldx;
@@ -163,7 +163,7 @@ template <class TE, class T, int RT> __global__ __launch_bounds__(256) void k_in
 template <class TE, class T, int RT, int VE, int WAVES> __global__ __launch_bounds__(WAVES * 64) void k_interact_bwd(InteractArgs g) {
     extern __shared__ float lds[];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-    const int64_t b = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const int64_t b = g.b0 + (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
     if (b >= g.B) return;
     constexpr int KB = RT <= 2 ? 1 : 4;                 // steps requested together
     const int stride = g.nf | 1, self = g.itself;
@@ -273,7 +273,7 @@ bool bad(const char *who, const InteractArgs &g, int te, int t) {
         set_error("%s: type codes %d, %d (embedding rows are float32 or of the output's type)", who, te, t);
         return true;
     }
-    if (g.B > INT32_MAX) { set_error("%s: batch of %lld", who, (long long)g.B); return true; }
+    if (g.B > ((int64_t)1 << 40)) { set_error("%s: batch of %lld", who, (long long)g.B); return true; }
     if (g.nf > 128 || g.nf < 1) { set_error("%s: %d feature rows, 1 .. 128 expected", who, g.nf); return true; }
     return false;
 }
@@ -290,8 +290,13 @@ template <class F> int by_types(int te, int t, F f) {
 
 template <class K> int launch(K kernel, const InteractArgs &g, size_t lds, hipStream_t st, int waves = 4) {
     if (lds > 65536) CAFE_HIP_CHECK(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.B + waves - 1) / waves)), dim3(64 * waves), lds, st, g);
-    CAFE_HIP_CHECK(hipGetLastError());
+    const int64_t most = (int64_t)1 << 24;                  // samples of a launch: a grid holds fewer than 2^32 work items
+    InteractArgs a = g;
+    for (a.b0 = 0; a.b0 < g.B; a.b0 += most) {
+        const int64_t n = g.B - a.b0 < most ? g.B - a.b0 : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((n + waves - 1) / waves)), dim3(64 * waves), lds, st, a);
+        CAFE_HIP_CHECK(hipGetLastError());
+    }
     return 0;
 }
 template <class TE, class T> int run_fwd(const InteractArgs &g, hipStream_t st) {

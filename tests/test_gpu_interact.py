@@ -200,3 +200,53 @@ def test_graph_and_streams():
             other = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+def test_a_batch_longer_than_a_launch():
+    b = 2 ** 24 + 77
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, emb = torch.randn(b, 3, device="cuda", generator=g), torch.randn(1, b, 3, device="cuda", generator=g)
+    xl, el = x.clone().requires_grad_(), emb.clone().requires_grad_()
+    out = dot_interaction(xl, el)
+    mag = (x.double().abs() * emb[0].double().abs()).sum(1)
+    check(out[:, 3].detach(), (x.double() * emb[0].double()).sum(1), (2 * 3 + 16) * U32 * mag + U32 * mag, "out")
+    dout = torch.randn(b, 4, device="cuda", generator=g)
+    dx, de = torch.autograd.grad(out, [xl, el], dout)
+    d = dout.double()
+    want, size = d[:, :3] + d[:, 3:] * emb[0].double(), d[:, :3].abs() + (d[:, 3:] * emb[0].double()).abs()
+    check(dx, want, (2 * 2 + 17) * U32 * size, "dx")
+    want = d[:, 3:] * x.double()
+    check(de[0], want, (2 * 2 + 17) * U32 * want.abs(), "demb")
+    torch.cuda.empty_cache()
+
+
+def test_offsets_past_32_bits():
+    """Rows of the last field start behind 2^32 bytes and 2^31 elements."""
+    f, b, d = 3, 700, 16
+    g = torch.Generator(device="cuda").manual_seed(0)
+    far = torch.empty(2 * (2 ** 30 + 2 ** 28) + b * d, device="cuda").as_strided((f, b, d), (2 ** 30 + 2 ** 28, d, 1))
+    x, emb, _ = make(f, b, d, torch.float32, torch.float32, True)
+    far.copy_(emb)
+    a, z = (dot_interaction(x, e.detach().requires_grad_()) for e in (emb, far))
+    assert torch.equal(a, z)
+    verify(x, far, False, torch.float32, g)
+    del far
+    torch.cuda.empty_cache()
+
+
+def test_wide_backward_in_a_graph():
+    """90 rows: the backward's LDS passes 64 KB, which the kernel is told of under capture too."""
+    x, emb, g = make(89, 40, 24, torch.float32, torch.float32, True)
+    xl, el = x.detach().requires_grad_(), emb.detach().requires_grad_()
+    dout = torch.randn(40, 24 + 90 * 89 // 2, device="cuda", generator=g)
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(dot_interaction(xl, el), [xl, el], dout)
+    for _ in range(3):
+        with torch.no_grad():
+            el.copy_(torch.randn(el.shape, device="cuda", generator=g))
+        want = torch.autograd.grad(dot_interaction(xl, el), [xl, el], dout)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(got, want))
