@@ -1,8 +1,8 @@
 """AdamW over many tensors in one launch (cafe_amd/csrc/cafe_adamw.hip), moments in 32 or 8 bits.
 
 The dense parameters of a head are a dozen tensors between one value and a few million; the reference steps them with
-torch.optim.  `AdamW` is a torch.optim.Optimizer; `adamw_step` the step itself over lists
-of tensors; `moment8_values` the float32 values that 8-bit moments stand for."""
+torch.optim.  `AdamW` is a torch.optim.Optimizer; `adamw_step` the step itself over lists of tensors; `moment8_values`
+the float32 values that 8-bit moments stand for."""
 import ctypes
 from typing import NamedTuple
 
@@ -60,8 +60,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     params: contiguous, of one type (float32, bfloat16, float16), on one GPU, no two sharing memory; grads: of the same
     type and shape.  exp_avgs, exp_avg_sqs: float32 tensors of the parameter's shape, or Moment8 throughout.  masters:
     None, or float32 tensors of the parameters' shapes that are updated in their place; the parameters then receive the
-    rounded values.  step: the number of this step, from 1; it is a number of the host, so a call under graph capture
-    takes `factors` instead (adamw_tick), a float32 tensor of three on the device.  All arithmetic is float32."""
+    rounded values (a float32 parameter may be its own master).  step: the number of this step, from 1; it is a number of
+    the host, so a call under graph capture takes `factors` instead (adamw_tick), a float32 tensor of three on the device.
+    All arithmetic is float32."""
     n = len(params)
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or (masters is not None and len(masters) != n):
         raise ValueError("params, grads, moments and masters are lists of one length")
@@ -92,9 +93,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     if masters is not None:
         _check(masters, torch.float32, index, shapes, "masters")
     cols += [zeros if masters is None else [w.data_ptr() for w in masters], counts]
-    used = [a for a, c in zip(cols[0], cols[7]) if c]
-    if len(set(used)) != len(used):
-        raise ValueError("a parameter is listed twice")
+    written = [a for f in (0, 2, 3, 4, 5) for a, c in zip(cols[f], counts) if c and a]
+    written += [a for a, p, c in zip(cols[6], cols[0], counts) if c and a and a != p]
+    if len(set(written)) != len(written):
+        raise ValueError("a parameter, moment or master is listed twice")
     on_device(first)
     if factors is None:
         if step is None or int(step) != step or step < 1:
@@ -110,6 +112,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
         _lib.check(_lib.load().cafe_adamw_dev(flat, n, DTYPE_CODE[dtype], 8 if eight else 32, float(lr), float(betas[0]), float(betas[1]),
                                               float(eps), float(weight_decay), step, None if factors is None else factors.data_ptr(), st),
                    "cafe_adamw_dev")
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])     # a backward that kept one says so
 
 
 def adamw_tick(step, factors, *, lr, betas=(0.9, 0.999), weight_decay=0.01):
@@ -174,6 +177,8 @@ class AdamW(torch.optim.Optimizer):
                                       master_weights=master_weights, capturable=capturable))
 
     def _init_state(self, p, group):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise _lib.CafeError("run one step with this parameter's gradient before the capture: replays would clear its moments")
         st = self.state[p]
         st["step"] = 0
         if group["state_bits"] == 8:
@@ -254,6 +259,7 @@ class AdamW(torch.optim.Optimizer):
                                  for k, v in state_dict["state"][i].items()}
         for group in self.param_groups:
             counts = group.pop("device_step", None)
-            if counts:
-                group["device_step"] = {k: (torch.full((1,), int(c), dtype=torch.int64, device=k),
-                                            torch.empty(3, dtype=torch.float32, device=k)) for k, c in counts.items()}
+            if counts:                          # resumed on another device: the count is the group's
+                devices = {p.device for p in group["params"]}
+                group["device_step"] = {str(d): (torch.full((1,), int(counts.get(str(d), max(counts.values()))), dtype=torch.int64, device=d),
+                                                 torch.empty(3, dtype=torch.float32, device=d)) for d in devices}

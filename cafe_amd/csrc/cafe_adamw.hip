@@ -31,6 +31,7 @@ constexpr int kItems = 48;              // tensors of one launch: their descript
 constexpr int lane_values(int bits) { return bits == 8 ? 8 : 4; }
 constexpr int span(int bits) { return 256 * lane_values(bits); }
 constexpr int kBlock = 256;
+constexpr int64_t kGrid = 1 << 22;      // workgroups of a launch (a grid holds fewer than 2^32 work items); longer tensors go in pieces
 
 struct Item { void *p; const void *g; void *m, *v; uint8_t *me, *ve; float *w; int64_t n; };
 struct AdamArgs {
@@ -246,17 +247,21 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
     a.b1 = (float)beta1; a.c1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.c2 = (float)(1.0 - beta2); a.eps = (float)eps;
     const hipStream_t st = (hipStream_t)stream;
     int i = 0;
+    int64_t from = 0;                   // values of tensor i that are behind us
     while (i < count) {
         int64_t blocks = 0;
         a.count = 0;
-        for (; i < count && a.count < kItems; i++) {
-            const int64_t n = tensors[7 * (int64_t)count + i], more = (n + span(state_bits) - 1) / span(state_bits);
-            if (n == 0) continue;
-            if (a.count && blocks + more > INT32_MAX) break;
-            auto at = [&](int f) { return (void *)(uintptr_t)tensors[f * (int64_t)count + i]; };
-            a.t[a.count] = Item{at(0), at(1), at(2), at(3), (uint8_t *)at(4), (uint8_t *)at(5), (float *)at(6), n};
+        while (i < count && a.count < kItems && blocks < kGrid) {
+            auto at = [&](int f) { return (uintptr_t)tensors[f * (int64_t)count + i]; };
+            auto on = [&](int f, int64_t bytes) { return at(f) ? (void *)(at(f) + bytes) : nullptr; };
+            const int64_t left = tensors[7 * (int64_t)count + i] - from, n = std::min<int64_t>(left, (kGrid - blocks) * span(state_bits));
+            if (left == 0) { i++; from = 0; continue; }
+            const int64_t e = from * (dtype == kF32 ? 4 : 2), s = state_bits == 8 ? from : from * 4;
+            a.t[a.count] = Item{on(0, e), on(1, e), on(2, s), on(3, s), (uint8_t *)on(4, from / kBlock), (uint8_t *)on(5, from / kBlock),
+                                (float *)on(6, from * 4), n};
             a.first[a.count++] = (int32_t)blocks;
-            blocks += more;
+            blocks += (n + span(state_bits) - 1) / span(state_bits);
+            from += n;
         }
         if (!a.count) break;
         a.first[a.count] = (int32_t)blocks;
@@ -293,18 +298,20 @@ extern "C" int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_s
     }
     ValueArgs a = {};
     int i = 0;
+    int64_t from = 0;
     while (i < count) {
         int64_t blocks = 0;
         a.count = 0;
-        for (; i < count && a.count < 2 * kItems; i++) {
+        while (i < count && a.count < 2 * kItems && blocks < kGrid) {
             auto at = [&](int f) { return tensors[f * (int64_t)count + i]; };
-            const int64_t n = at(3), more = (n + span(8) - 1) / span(8);
-            if (n == 0) continue;
-            if (a.count && blocks + more > INT32_MAX) break;
-            a.t[a.count] = ValueItem{(const uint8_t *)(uintptr_t)at(0), (const uint8_t *)(uintptr_t)at(1), (float *)(uintptr_t)at(2), n};
+            const int64_t left = at(3) - from, n = std::min<int64_t>(left, (kGrid - blocks) * span(8));
+            if (left == 0) { i++; from = 0; continue; }
+            a.t[a.count] = ValueItem{(const uint8_t *)(uintptr_t)at(0) + from, (const uint8_t *)(uintptr_t)at(1) + from / kBlock,
+                                     (float *)(uintptr_t)at(2) + from, n};
             a.second[a.count] = at(4) != 0;
             a.first[a.count++] = (int32_t)blocks;
-            blocks += more;
+            blocks += (n + span(8) - 1) / span(8);
+            from += n;
         }
         if (!a.count) break;
         a.first[a.count] = (int32_t)blocks;

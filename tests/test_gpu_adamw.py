@@ -308,3 +308,61 @@ def test_tick():
         # the double's powers are good to a few 2^-52, 1 - 0.99 loses two digits of that: float32's half step remains
         near(factors.cpu(), want, 1.01 * U32 * want, "factors")
         assert int(step) == t
+
+
+def test_a_capture_creates_no_moments():
+    """Zeros written in a capture would be written again by every replay."""
+    p, late = (torch.nn.Parameter(torch.ones(10, device="cuda")) for _ in range(2))
+    opt = AdamW([p, late], capturable=True)
+    p.grad = torch.ones(10, device="cuda")
+    opt.step()
+    late.grad = torch.ones(10, device="cuda")
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), pytest.raises(Exception, match="before the capture"):
+        opt.step()
+    opt.step()                                                                       # eager: creates them
+    assert len(opt.state[late]) > 1
+
+
+def test_a_backward_notices_the_step():
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    loss = (p * p).sum()
+    adamw_step([p.detach()], [torch.ones(4, device="cuda")], [torch.zeros(4, device="cuda")], [torch.zeros(4, device="cuda")], step=1, lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("t,bits", [(torch.bfloat16, 8), (torch.float32, 32)])
+def test_tensors_longer_than_a_launch(t, bits):
+    """2^22 workgroups of 2048 (8 bits) or 1024 values and a few more: repeated rows get what one row gets, in every piece."""
+    row, rows = 256 * 4097, 8200 if bits == 8 else 4100
+    assert row * rows > 2 ** 22 * (2048 if bits == 8 else 1024)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    small = [torch.randn(row, device="cuda", generator=g).to(t) for _ in range(2)]
+    def spread(x):
+        return x.repeat(rows)
+    p, grad = (spread(x) for x in small)
+    if bits == 8:
+        ms, ml = ([Moment8.zeros(n, "cuda") for _ in range(2)] for n in (row, row * rows))
+        ws, wl = [small[0].float()], [p.float()]
+    else:
+        ms, ml = ([torch.zeros(n, device="cuda") for _ in range(2)] for n in (row, row * rows))
+        ws = wl = None
+    for step in (1, 2):
+        adamw_step([small[0]], [small[1]], [ms[0]], [ms[1]], step=step, masters=ws, **HYPER)
+        adamw_step([p], [grad], [ml[0]], [ml[1]], step=step, masters=wl, **HYPER)
+
+    def same(long, one):
+        return all(torch.equal(r, one) for r in long.view(rows, -1))
+    assert same(p, small[0])
+    if bits == 8:
+        assert same(wl[0], ws[0]) and all(same(a, b) for k in range(2) for a, b in zip(ml[k], ms[k]))
+        del p, grad, wl
+        (lm,), (lv,) = moment8_values([ml[0]], [ml[1]])
+        (sm,), (sv,) = moment8_values([ms[0]], [ms[1]])
+        assert same(lm, sm) and same(lv, sv)
+    else:
+        assert same(ml[0], ms[0]) and same(ml[1], ms[1])
+    p = grad = wl = ml = lm = lv = None
+    torch.cuda.empty_cache()

@@ -128,3 +128,23 @@ def test_c_entry_points():
     assert L.cafe_moment8_values_dev(None, 1, None) != 0
     assert L.cafe_moment8_values_dev((ctypes.c_int64 * 5)(0, 4096, 4096, 3, 0), 1, None) != 0
     assert L.cafe_moment8_values_dev((ctypes.c_int64 * 5)(4096, 4096, 4096, -3, 0), 1, None) != 0
+
+
+def test_nothing_is_listed_twice():
+    z = lambda: torch.zeros(5)                                                         # noqa: E731
+    p, m = z(), z()
+    for lists in (([p, p], [z(), z()], [z(), z()], [z(), z()]), ([z(), z()], [z(), z()], [m, m], [z(), z()]),
+                  ([z(), z()], [z(), z()], [m, z()], [z(), m])):
+        with pytest.raises(ValueError, match="twice"):
+            adamw_step(*lists, step=1, lr=0.1)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([z(), z()], [z(), z()], [z(), z()], [z(), z()], step=1, lr=0.1, masters=[m, m])
+
+
+def test_the_step_count_follows_a_group_to_another_device():
+    opt = AdamW([torch.nn.Parameter(torch.zeros(3))], capturable=True)
+    saved = opt.state_dict()
+    saved["param_groups"][0]["device_step"] = {"cuda:5": 7}
+    opt.load_state_dict(saved)
+    assert list(opt.param_groups[0]["device_step"]) == ["cpu"]
+    assert opt.state_dict()["param_groups"][0]["device_step"] == {"cpu": 7}
