@@ -3,10 +3,10 @@
 //     m = b1 m + (1 - b1) g     v = b2 v + (1 - b2) g^2
 //     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// for the dense parameters of the models' heads (the reference steps them
-// with torch.optim).  All arithmetic is float32, operation by operation as written (no contraction), so the
-// 8-bit codes do not depend on how a compiler fuses.  Bound by memory: 28 bytes per float32 value with float32 moments,
-// 16 with 8-bit ones.
+// for the dense parameters of the models' heads (the reference steps them with torch.optim).  All arithmetic is float32,
+// operation by operation as written (no contraction), so the 8-bit codes do not depend on how a compiler fuses.  Bound by
+// memory: 28 bytes per float32 value with float32 moments, 16 with 8-bit ones; 36 M bfloat16 values with 8-bit moments and
+// master weights (18 bytes each) take 127-140 us, 4.6-5.1 TB/s, and reading the moments out as float32 (10 bytes) 88-95.
 //
 // 8-bit moments.  256 consecutive values share an exponent E, that of the largest finite magnitude among them (at least
 // -126; stored plus 127).  A value is scaled by 2^-E -- exactly -- into [0, 2) and rounded to nearest even in a small
