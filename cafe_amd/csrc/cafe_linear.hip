@@ -688,15 +688,15 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 // out and back (2.5 TB/s) and the slices.  The constants are fitted to 1700 timings of 45 products between 1 x 256 x 8192
 // and 16384 x 3341 x 256 in float32 and bfloat16; the choice is within 1.2 % of the fastest on average and 25 % off at
 // worst (1 x 256 outputs over 8192 in bfloat16).  Both sides of it, bfloat16: 8192 x 256 outputs over 512 take 8.0 us in
-// 64 x 64 tiles, 10.5 in 128 x 128 (half the units idle), 12.6 in 256 x 128; 8192 x 1024 over 1024 (dx) take 34.8, 28.2 and
-// 24.7; in float32 256 x 128 gains 2 % there and loses 5 % in slices.  float32: 64 x 256 outputs over 8192 take 14.7 us in
+// 64 x 64 tiles, 9.6 in 128 x 128 (half the units idle), 12.6 in 256 x 128; 8192 x 1024 over 1024 (dx) take 33.4, 28.4 and
+// 22.9; in float32 256 x 128 gains 2 % there and loses 5 % in slices.  float32: 64 x 256 outputs over 8192 take 14.7 us in
 // 32 slices and 22 in 12, 128 x 367 over 367 take 9.6 in 4 and 11.9 in 12.
 struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; double us; };
 struct Cost { double shared[4], alone[4], ends, join, per_slice, launch; };
 
 Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
     static const Cost f32 = {{0, 1.85, 1.01, 0.54}, {0, 2.25, 1.25, 0.68}, 2.4, 1.8, 0.05, 4.8};
-    static const Cost half = {{0.94, 0.6, 0.41, 0.28}, {0.94, 0.785, 0.56, 0.315}, 1.4, 2.2, 0.14, 4.6};
+    static const Cost half = {{0.92, 0.665, 0.49, 0.27}, {0.98, 0.665, 0.49, 0.293}, 1.25, 2.5, 0.13, 4.55};
     static const struct { int bm, bn, kind; } tiles[] = {{256, 128, 0}, {128, 128, 1}, {128, 64, 2}, {64, 128, 2}, {64, 64, 3}};
     const Cost &c = dtype == kF32 ? f32 : half;
     const int64_t bk = 128 / elem_size(dtype), kts = (R + bk - 1) / bk;
@@ -729,9 +729,13 @@ template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, 
             return 0;
         }
     }
-    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128, 2, 2>), grid, dim3(256), 0, st, g);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64, 2, 2>), grid, dim3(256), 0, st, g);
-    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128, 2, 2>), grid, dim3(256), 0, st, g);
+    // Eight waves where 16-bit types leave each two 32 x 32 blocks (one, in half tiles): the four products of a step are
+    // too short to cover a wave's own waits, a second wave on the unit does (16384 x 3341 x 256 in bfloat16 47.8 us, with
+    // four waves 51.3; 8192 x 1024 outputs over 479 across rows 15.9 and 19.6).  float32 with eight waves loses 4-10 % in dx.
+    constexpr int W = sizeof(T) == 2 ? 2 : 1;
+    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64, 2 * W, 2>), grid, dim3(256 * W), 0, st, g);
+    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
     else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
