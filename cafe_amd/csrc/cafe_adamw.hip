@@ -6,7 +6,7 @@
 // for the dense parameters of the models' heads (the reference steps them with torch.optim).  All arithmetic is float32,
 // operation by operation as written (no contraction), so the 8-bit codes do not depend on how a compiler fuses.  Bound by
 // memory: 28 bytes per float32 value with float32 moments, 16 with 8-bit ones; 36 M bfloat16 values with 8-bit moments and
-// master weights (18 bytes each) take 127-140 us, 4.6-5.1 TB/s, and reading the moments out as float32 (10 bytes) 88-95.
+// master weights (18 bytes each) take 125-134 us, 4.8-5.2 TB/s, and reading the moments out as float32 (10 bytes) 71.
 //
 // 8-bit moments.  256 consecutive values share an exponent E, that of the largest finite magnitude among them (at least
 // -126; stored plus 127).  A value is scaled by 2^-E -- exactly -- into [0, 2) and rounded to nearest even in a small
@@ -45,9 +45,34 @@ static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
 // L elements, at element alignment, as float or int; from `n` on nothing is touched and zeros are read
 template <class T, int L> struct __attribute__((packed, aligned(sizeof(T)))) Lane { T e[L]; };
-template <int L, class T, class F> __device__ __forceinline__ void get(const T *p, int n, F *out) {
+// Past the caches (PAST): what is read or written so is not kept there.
+typedef uint32_t past4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t past2 __attribute__((ext_vector_type(2), aligned(1)));
+template <bool PAST, class U> __device__ __forceinline__ U load_lane(const U *p) {
+    if constexpr (!PAST) return *p;
+    else if constexpr (sizeof(U) == 8) return __builtin_bit_cast(U, __builtin_nontemporal_load((const past2 *)p));
+    else {
+        static_assert(sizeof(U) % 16 == 0, "");
+        union { U u; past4 v[sizeof(U) / 16]; } x;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(U) / 16); i++) x.v[i] = __builtin_nontemporal_load((const past4 *)p + i);
+        return x.u;
+    }
+}
+template <bool PAST, class U> __device__ __forceinline__ void store_lane(U *p, U u) {
+    if constexpr (!PAST) *p = u;
+    else if constexpr (sizeof(U) == 8) __builtin_nontemporal_store(__builtin_bit_cast(past2, u), (past2 *)p);
+    else {
+        static_assert(sizeof(U) % 16 == 0, "");
+        union { U u; past4 v[sizeof(U) / 16]; } x;
+        x.u = u;
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(U) / 16); i++) __builtin_nontemporal_store(x.v[i], (past4 *)p + i);
+    }
+}
+template <int L, bool PAST, class T, class F> __device__ __forceinline__ void get(const T *p, int n, F *out) {
     if (n >= L) {
-        const Lane<T, L> u = *(const Lane<T, L> *)p;
+        const Lane<T, L> u = load_lane<PAST>((const Lane<T, L> *)p);
 #pragma unroll
         for (int i = 0; i < L; i++) out[i] = (F)u.e[i];
     } else {
@@ -55,11 +80,11 @@ template <int L, class T, class F> __device__ __forceinline__ void get(const T *
         for (int i = 0; i < L; i++) out[i] = i < n ? (F)p[i] : (F)0;
     }
 }
-template <int L, class T, class F> __device__ __forceinline__ void put(T *p, int n, const F *in) {
+template <int L, bool PAST, class T, class F> __device__ __forceinline__ void put(T *p, int n, const F *in) {
     Lane<T, L> u;
 #pragma unroll
     for (int i = 0; i < L; i++) u.e[i] = (T)in[i];
-    if (n >= L) *(Lane<T, L> *)p = u;
+    if (n >= L) store_lane<PAST>((Lane<T, L> *)p, u);
     else {
 #pragma unroll
         for (int i = 0; i < L; i++)
@@ -117,7 +142,9 @@ __device__ __forceinline__ int item_of(const int32_t *first, int count, int bloc
     return lo;
 }
 
-template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
+// PAST: a step over more than the caches hold.  Nothing of it is found there by the next step, so moments, masters and
+// gradients go past them and leave the room to the parameters, which the next forward reads.
+template <class T, bool BITS8, bool PAST> __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
     const int k = item_of(a.first, a.count, blockIdx.x);
     const Item t = a.t[k];
     float step_size = a.step_size, root = a.root, keep = a.keep;
@@ -127,19 +154,19 @@ template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(Ad
     if (block * kBlock >= t.n) return;                  // the block's 32 lanes leave together
     const int n = (int)(t.n - at < L ? t.n - at : L);          // may be <= 0
     float p[L], g[L], m[L], v[L];
-    get<L>((const T *)t.g + at, n, g);
-    if (t.w) get<L>(t.w + at, n, p);
-    else get<L>((const T *)t.p + at, n, p);
-    if (BITS8) {
+    get<L, PAST>((const T *)t.g + at, n, g);
+    if (t.w) get<L, PAST>(t.w + at, n, p);
+    else get<L, PAST>((const T *)t.p + at, n, p);
+    if constexpr (BITS8) {
         int cm[L], cv[L];
-        get<L>((const uint8_t *)t.m + at, n, cm);
-        get<L>((const uint8_t *)t.v + at, n, cv);
+        get<L, PAST>((const uint8_t *)t.m + at, n, cm);
+        get<L, PAST>((const uint8_t *)t.v + at, n, cv);
         const int em = (int)t.me[block] - 127, ev = (int)t.ve[block] - 127;
 #pragma unroll
         for (int i = 0; i < L; i++) { m[i] = decode8<false>(cm[i], em); v[i] = decode8<true>(cv[i], ev); }
     } else {
-        get<L>((const float *)t.m + at, n, m);
-        get<L>((const float *)t.v + at, n, v);
+        get<L, PAST>((const float *)t.m + at, n, m);
+        get<L, PAST>((const float *)t.v + at, n, v);
     }
 #pragma unroll
     for (int i = 0; i < L; i++) {
@@ -148,7 +175,7 @@ template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(Ad
         const float denom = sqrtf(v[i]) * root + a.eps;
         p[i] = p[i] * keep - (m[i] / denom) * step_size;
     }
-    if (BITS8) {
+    if constexpr (BITS8) {
 #pragma unroll
         for (int i = 0; i < L; i++)
             if (i >= n) m[i] = v[i] = 0.f;
@@ -156,15 +183,15 @@ template <class T, bool BITS8> __global__ __launch_bounds__(256) void k_adamw(Ad
         block_exponents(m, v, &em, &ev);
 #pragma unroll
         for (int i = 0; i < L; i++) { cm[i] = encode8<false>(m[i], em); cv[i] = encode8<true>(v[i], ev); }
-        put<L>((uint8_t *)t.m + at, n, cm);
-        put<L>((uint8_t *)t.v + at, n, cv);
+        put<L, PAST>((uint8_t *)t.m + at, n, cm);
+        put<L, PAST>((uint8_t *)t.v + at, n, cv);
         if ((threadIdx.x & 31) == 0) { t.me[block] = (uint8_t)(em + 127); t.ve[block] = (uint8_t)(ev + 127); }
     } else {
-        put<L>((float *)t.m + at, n, m);
-        put<L>((float *)t.v + at, n, v);
+        put<L, PAST>((float *)t.m + at, n, m);
+        put<L, PAST>((float *)t.v + at, n, v);
     }
-    if (t.w) put<L>(t.w + at, n, p);
-    put<L>((T *)t.p + at, n, p);
+    if (t.w) put<L, PAST>(t.w + at, n, p);
+    put<L, false>((T *)t.p + at, n, p);
 }
 
 struct ValueItem { const uint8_t *codes, *exps; float *out; int64_t n; };
@@ -176,7 +203,7 @@ struct ValueArgs {
 };
 static_assert(sizeof(ValueArgs) <= 4096, "kernel arguments");
 
-__global__ __launch_bounds__(256) void k_moment_values(ValueArgs a) {
+template <bool PAST> __global__ __launch_bounds__(256) void k_moment_values(ValueArgs a) {
     const int k = item_of(a.first, a.count, blockIdx.x);
     const ValueItem t = a.t[k];
     const bool second = a.second[k];
@@ -186,10 +213,10 @@ __global__ __launch_bounds__(256) void k_moment_values(ValueArgs a) {
     const int n = (int)(t.n - at < L ? t.n - at : L), e = (int)t.exps[at / kBlock] - 127;
     int c[L];
     float v[L];
-    get<L>(t.codes + at, n, c);
+    get<L, PAST>(t.codes + at, n, c);
 #pragma unroll
     for (int i = 0; i < L; i++) v[i] = second ? decode8<true>(c[i], e) : decode8<false>(c[i], e);
-    put<L>(t.out + at, n, v);
+    put<L, PAST>(t.out + at, n, v);
 }
 
 __global__ void k_adamw_tick(int64_t *step, const float *lr_dev, double lr, double b1, double b2, double wd, float *factors) {
@@ -209,8 +236,15 @@ bool bad_hyper(const char *who, double lr, double b1, double b2, double eps, dou
     return false;
 }
 
-template <class T, bool BITS8> int launch(const AdamArgs &a, unsigned blocks, hipStream_t st) {
-    hipLaunchKernelGGL((k_adamw<T, BITS8>), dim3(blocks), dim3(256), 0, st, a);
+// Bytes of a call from which its arrays go past the caches (256 MB behind the L2s).  A step, with gradients just written
+// and parameters read afterwards: 19 M float32 values with float32 moments (528 MB) 133 us, 146 through the caches, 29 M
+// 218 and 247, 38 M bfloat16 ones with 8-bit moments and masters (680 MB) 201 and 230; below, 15 M float32 values (411 MB)
+// take 115 and 95, 25 M bfloat16 ones (453 MB) 160 and 138.  Reading 38 M moments out twice (302 MB): 71 and 92 us.
+constexpr int64_t kPastStep = (int64_t)480 << 20, kPastValues = (int64_t)256 << 20;
+
+template <class T, bool BITS8> int launch(const AdamArgs &a, unsigned blocks, bool past, hipStream_t st) {
+    if (past) hipLaunchKernelGGL((k_adamw<T, BITS8, true>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_adamw<T, BITS8, false>), dim3(blocks), dim3(256), 0, st, a);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -246,6 +280,11 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
     }
     a.b1 = (float)beta1; a.c1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.c2 = (float)(1.0 - beta2); a.eps = (float)eps;
     const hipStream_t st = (hipStream_t)stream;
+    int64_t bytes = 0;
+    for (int k = 0; k < count; k++)
+        bytes += tensors[7 * (int64_t)count + k] * ((dtype == kF32 ? 4 : 2) * (tensors[6 * (int64_t)count + k] ? 2 : 3) +
+                                                    (tensors[6 * (int64_t)count + k] ? 8 : 0) + (state_bits == 8 ? 4 : 16));
+    const bool past = bytes > kPastStep;
     int i = 0;
     int64_t from = 0;                   // values of tensor i that are behind us
     while (i < count) {
@@ -268,9 +307,9 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
         const unsigned b = (unsigned)blocks;
         const bool s8 = state_bits == 8;
         int rc;
-        if (dtype == kF32) rc = s8 ? launch<float, true>(a, b, st) : launch<float, false>(a, b, st);
-        else if (dtype == kBF16) rc = s8 ? launch<__bf16, true>(a, b, st) : launch<__bf16, false>(a, b, st);
-        else rc = s8 ? launch<_Float16, true>(a, b, st) : launch<_Float16, false>(a, b, st);
+        if (dtype == kF32) rc = s8 ? launch<float, true>(a, b, past, st) : launch<float, false>(a, b, past, st);
+        else if (dtype == kBF16) rc = s8 ? launch<__bf16, true>(a, b, past, st) : launch<__bf16, false>(a, b, past, st);
+        else rc = s8 ? launch<_Float16, true>(a, b, past, st) : launch<_Float16, false>(a, b, past, st);
         if (rc) return rc;
     }
     return 0;
@@ -296,6 +335,9 @@ extern "C" int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_s
             return 1;
         }
     }
+    int64_t bytes = 0;
+    for (int k = 0; k < count; k++) bytes += 4 * tensors[3 * (int64_t)count + k];
+    const bool past = bytes > kPastValues;
     ValueArgs a = {};
     int i = 0;
     int64_t from = 0;
@@ -315,7 +357,8 @@ extern "C" int cafe_moment8_values_dev(const int64_t *tensors, int count, cafe_s
         }
         if (!a.count) break;
         a.first[a.count] = (int32_t)blocks;
-        hipLaunchKernelGGL(k_moment_values, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+        if (past) hipLaunchKernelGGL(k_moment_values<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL(k_moment_values<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
         CAFE_HIP_CHECK(hipGetLastError());
     }
     return 0;

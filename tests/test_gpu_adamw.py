@@ -366,3 +366,36 @@ def test_tensors_longer_than_a_launch(t, bits):
         assert same(ml[0], ms[0]) and same(ml[1], ms[1])
     p = grad = wl = ml = lm = lv = None
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("t", TYPES)
+def test_steps_past_the_caches(t, bits, master):
+    """More than 480 MB in a call: the arrays go past the caches, from addresses off any 16-byte boundary too; repeated rows
+    get what one row gets."""
+    row, rows = 256 * 4097, 52
+    g = torch.Generator(device="cuda").manual_seed(1)
+    small = [torch.randn(row, device="cuda", generator=g).to(t) for _ in range(2)]
+
+    def spread(x):
+        out = torch.empty(row * rows + 1, dtype=x.dtype, device="cuda")[1:]
+        out.view(rows, row).copy_(x)
+        return out
+
+    def moments(n):
+        return [Moment8.zeros(n, "cuda") if bits == 8 else torch.zeros(n, device="cuda") for _ in range(2)]
+    (p, grad), ms, ml = [spread(x) for x in small], moments(row), moments(row * rows)
+    ws, wl = ([small[0].float().clone()], [spread(small[0].float())]) if master else (None, None)
+    for step in (1, 2):
+        adamw_step([small[0]], [small[1]], [ms[0]], [ms[1]], step=step, masters=ws, **HYPER)
+        adamw_step([p], [grad], [ml[0]], [ml[1]], step=step, masters=wl, **HYPER)
+    pairs = [(p, small[0])] + ([(wl[0], ws[0])] if master else [])
+    if bits == 8:
+        lv, sv = moment8_values([ml[0]], [ml[1]]), moment8_values([ms[0]], [ms[1]])
+        pairs += [(a[0], b[0]) for a, b in zip(lv, sv)] + [(a, b) for k in range(2) for a, b in zip(ml[k], ms[k])]
+    else:
+        pairs += list(zip(ml, ms))
+    for long, one in pairs:
+        assert (long.view(rows, -1) == one).all()
+    torch.cuda.empty_cache()
