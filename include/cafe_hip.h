@@ -324,7 +324,8 @@ void cafe_ae_ref_update(int idx);
  *     parameters.  Same contract as (B): device pointers, a stream, nothing allocated, nothing synchronised, no state
  *     kept between calls; workspaces are the caller's (sizes from the *_ws functions, contents undefined before and
  *     after), one per call in flight.  All calls may be captured into a HIP graph.  Type codes: 0 float32, 1 bfloat16,
- *     2 float16.  Row strides (ld*) are in elements; rows need no alignment beyond their elements'.
+ *     2 float16.  Row strides (ld*) are in elements; rows need no alignment beyond their elements'.  What a call writes
+ *     overlaps nothing that it reads, nor another output.
  * ------------------------------------------------------------------------------------------------ */
 /* y[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + res[M, N], all of one type, sums in float32 (dlrm_s_pytorch.py:213-251:
  * a Linear and its activation; wdl.py:704-721: the last deep layer with the wide part's logit as `res`).
