@@ -316,10 +316,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
         }
     };
     // Registers of set u -> LDS buffer of tile kt.
-    auto stage = [&](int64_t kt, int u, bool woven) {
+    auto stage = [&](int64_t kt, int u, bool woven, bool sums) {
         char *la = lds + (kt & 1) * STAGE, *lb = la + OA::BYTES;
         if (!woven) { A.align(ra[u]); B.align(rb[u]); }
-        if (!woven && sums) {
+        if (sums) {
 #pragma unroll
             for (int n = 0; n < OA::N; n++) {
                 float v[E];
@@ -342,14 +342,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
     // Tile kt: its first fragments are in set 0.  The next tile goes to LDS behind step 1, the barrier stands behind step
     // 2, and the next tile's first fragments are fetched before step 3's products: the matrix unit always has a step's
     // worth of work while LDS answers.
-    // INNER: every tile it touches lies inside the operands and the slice; WOVEN: nor has a chunk to be shifted or a column
-    // to be summed, so that no branch stands between the products.
+    // INNER: every tile it touches lies inside the operands and the slice; WOVEN: nor has a chunk to be shifted, and SUMS
+    // says whether columns are summed, so that no branch stands between the products (decided at run time instead, sums
+    // cost 8192 x 1024 x 1024 in float32 15 us).
     constexpr int MF = TI * TJ * (sizeof(T) == 4 ? 4 : 1), FR = TI * (ACOLS ? 2 : 1) + TJ * (BCOLS ? 2 : 1), MV = OA::N + OB::N;
     auto body = [&](int64_t kt, int u, auto mode) {
-        constexpr bool INNER = decltype(mode)::value > 0, WOVEN = decltype(mode)::value == 2;
+        constexpr bool INNER = decltype(mode)::value > 0, WOVEN = decltype(mode)::value >= 2, SUMS = decltype(mode)::value == 3;
         const int un = (u + 1) % PF;
         fetch(kt, 1, 1);
-        if (INNER || kt + 1 < k1) stage(kt + 1, un, WOVEN);
+        if (INNER || kt + 1 < k1) stage(kt + 1, un, WOVEN, WOVEN ? SUMS : sums);
         mfma_step<T, TI, TJ>(fa[0], fb[0], acc);
         if constexpr (WOVEN) weave<MF, FR, MV, 0>();
         __builtin_amdgcn_sched_barrier(0);
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
         mfma_step<T, TI, TJ>(fa[1], fb[1], acc);
     };
     if (k0 < k1) {
-        const bool woven = !(sums || A.edge() || B.edge());
+        const bool woven = !(A.edge() || B.edge());
         // tiles that the inner bodies may request: all but the reduction's last, none where rows are shorter than a chunk
         const int64_t inner = A.tiny || B.tiny ? k0 : k1 < kts ? k1 : kts - 1;
         int64_t kt = k0;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
                     request(k0 + u, u, IN);
                     __builtin_amdgcn_sched_barrier(0);          // in this order: the loop waits for the older set
                 }
-            stage(k0, 0, decltype(mode)::value == 2);
+            stage(k0, 0, decltype(mode)::value >= 2, sums);
             if (IN || k0 + PF < k1) request(k0 + PF, 0, IN);
             __syncthreads();
             fetch(k0, 0, 0);
@@ -391,8 +392,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             }
         };
         if (k0 + 2 * PF >= inner) start(std::integral_constant<int, 0>{});
-        else if (woven) run(std::integral_constant<int, 2>{});
-        else if constexpr (ACOLS || BCOLS) run(std::integral_constant<int, 1>{});
+        else if (woven && !sums) run(std::integral_constant<int, 2>{});
+        else if constexpr (ACOLS && BCOLS) {
+            constexpr int WITH_SUMS = BM < 256 ? 3 : 1;             // 3 would spill registers in the largest tile
+            if (woven) run(std::integral_constant<int, WITH_SUMS>{});
+            else run(std::integral_constant<int, 1>{});
+        } else if constexpr (BCOLS) run(std::integral_constant<int, 1>{});
         for (; kt < k1; kt += PF) {
 #pragma unroll
             for (int u = 0; u < PF; u++)
