@@ -102,6 +102,7 @@ struct Out {
 struct TileArgs {
     const void *a, *b;
     int64_t lda, ldb;
+    int64_t low;                      // != 0: A stands for A + what lies that many elements behind it
     int64_t I, J, R;                  // C is [I, J], the reduction runs over R
     float *sums; void *sums_out;      // column sums of A: per slice, or (one slice) the result itself; null: not wanted
     int tiles_j, tiles;               // tiles along j, tiles in all
@@ -313,7 +314,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
     const int tile = xcd_tile(blockIdx.x, g.tiles);
     const int64_t i0 = (int64_t)(tile / g.tiles_j) * BM, j0 = (int64_t)(tile % g.tiles_j) * BN;
     const int64_t kts = (g.R + BK - 1) / BK;
-    const int64_t k0 = kts * blockIdx.y / g.slices, k1 = kts * (blockIdx.y + 1) / g.slices;
+    const bool second = (int)blockIdx.y >= g.slices;                       // slices of A's second part (g.low), over the same B
+    const int slice = blockIdx.y - (second ? g.slices : 0);
+    const int64_t k0 = kts * slice / g.slices, k1 = kts * (slice + 1) / g.slices;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
     f32x16 acc[TI][TJ];
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             for (int e = 0; e < 16; e++) acc[a][b][e] = 0.f;
     OA A;
     OB B;
-    A.init(g.a, g.lda, g.I, g.R, i0);
+    A.init((const T *)g.a + (second ? g.low : 0), g.lda, g.I, g.R, i0);
     B.init(g.b, g.ldb, g.J, g.R, j0);
     u32x4 ra[PF][OA::N], rb[PF][OB::N];
     const bool sums = ACOLS && BCOLS && g.sums && j0 == 0;
@@ -647,9 +650,9 @@ template <class T, int FT, int WAVES, bool MANY_W> __global__ __launch_bounds__(
 
 // dz = dy * act'(z), rounded.  kept: z in the type (relu: anything of its sign), or the slopes in float32.  One 16-byte
 // chunk per thread and step.  SUMS: the column sums of the unrounded values over the block's rows, a row of `sums` per
-// blockIdx.y; a block then has `lanes` chunks side by side.  Bound by memory: 8192 x 1024 in float32 takes 15.3 us (6.5
+// blockIdx.y; a block then has `lanes` chunks side by side.  LOW: what the rounding left, rounded, `low` values further.  Bound by memory: 8192 x 1024 in float32 takes 15.3 us (6.5
 // TB/s, cached in part), 16384 x 256 in bfloat16 with float32 slopes and sums 10.2 (3.3 TB/s; 7 without the sums).
-template <class T, int ACT> __device__ __forceinline__ void dz_chunk(const T *dy, const void *kept, int64_t at_kept, T *dz, int left, float *g) {
+template <class T, int ACT, bool LOW> __device__ __forceinline__ void dz_chunk(const T *dy, const void *kept, int64_t at_kept, T *dz, int64_t low, int left, float *g) {
     constexpr int E = Elem<T>::per_chunk;
     float k[E];
     unpack<T>(load_some(dy, left), g);
@@ -661,20 +664,28 @@ template <class T, int ACT> __device__ __forceinline__ void dz_chunk(const T *dy
     }
 #pragma unroll
     for (int e = 0; e < E; e++) g[e] = through<ACT>(g[e], k[e]);
-    store_some(dz, pack<T>(g), left);
+    const u32x4 high = pack<T>(g);
+    store_some(dz, high, left);
+    if constexpr (LOW) {
+        float h[E];
+        unpack<T>(high, h);
+#pragma unroll
+        for (int e = 0; e < E; e++) h[e] = fabsf(h[e]) < INFINITY ? g[e] - h[e] : 0.f;
+        store_some(dz + low, pack<T>(h), left);
+    }
 }
-template <class T, int ACT>
-__global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t M, int64_t N) {
+template <class T, int ACT, bool LOW>
+__global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t low, int64_t M, int64_t N) {
     constexpr int E = Elem<T>::per_chunk;
     const int64_t chunks = (N + E - 1) / E, n = M * chunks;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
         const int64_t m = q / chunks, col = (q - m * chunks) * E;
         float g[E];
-        dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, (int)(N - col < E ? N - col : E), g);
+        dz_chunk<T, ACT, LOW>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, (int)(N - col < E ? N - col : E), g);
     }
 }
-template <class T, int ACT>
-__global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t M, int64_t N,
+template <class T, int ACT, bool LOW>
+__global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t low, int64_t M, int64_t N,
                                                 int lanes, int64_t rows, float *sums) {
     constexpr int E = Elem<T>::per_chunk;
     __shared__ float red[256 * E];
@@ -688,7 +699,7 @@ __global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const
 #pragma unroll 4
         for (int64_t m = blockIdx.y * rows + y; m < m1; m += ny) {
             float g[E];
-            dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, left, g);
+            dz_chunk<T, ACT, LOW>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, left, g);
 #pragma unroll
             for (int e = 0; e < E; e++) s[e] += g[e];
         }
@@ -754,7 +765,7 @@ template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, 
         set_error("cafe_linear: %lld tiles of %d x %d are more than a launch takes", (long long)p.tiles, p.bm, p.bn);
         return 1;
     }
-    const dim3 grid((unsigned)g.tiles, (unsigned)p.slices);
+    const dim3 grid((unsigned)g.tiles, (unsigned)(p.slices * (g.low ? 2 : 1)));
     if constexpr (sizeof(T) == 2) {
         if (p.bm == 256) {
             hipLaunchKernelGGL((k_tile<T, AC, BC, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
@@ -786,14 +797,14 @@ template <class F> void with_act(int act, F f) {
 }
 
 // Joins a product's slices and `parts` rows of column sums (either may be missing).
-template <class T> int join(const Plan &p, const TileArgs &g, const Out &o, float *part, const float *sums, int parts, T *sums_out, hipStream_t st) {
+template <class T> int join(int slices, const TileArgs &g, const Out &o, float *part, const float *sums, int parts, T *sums_out, hipStream_t st) {
     constexpr int E = Elem<T>::per_chunk;
     Out j = o;
     j.part = part;
     const int out_blocks = part ? (int)std::min<int64_t>((g.I * ((g.J + E - 1) / E) + 255) / 256, 256 * 16) : 0;
     const int sum_blocks = sums_out ? (int)std::min<int64_t>((g.I + 15) / 16, 1 << 16) : 0;
     with_act(o.act, [&](auto a) {
-        hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3((unsigned)(out_blocks + sum_blocks)), dim3(256), 0, st, j, g.I, g.J, p.slices,
+        hipLaunchKernelGGL((k_join<T, decltype(a)::value>), dim3((unsigned)(out_blocks + sum_blocks)), dim3(256), 0, st, j, g.I, g.J, slices,
                            out_blocks, sums, parts, sums_out);
     });
     CAFE_HIP_CHECK(hipGetLastError());
@@ -806,7 +817,7 @@ template <class T, bool AC, bool BC>
 int product(const Plan &p, TileArgs g, float *part, float *sums, int parts, T *sums_out, hipStream_t st) {
     if (g.I == 0 || (g.J == 0 && !sums_out)) return 0;
     const bool out = g.o.y != nullptr && g.J > 0;
-    if (!out && parts) return join<T>(p, g, g.o, nullptr, sums, parts, sums_out, st);
+    if (!out && parts) return join<T>(0, g, g.o, nullptr, sums, parts, sums_out, st);
     if (!out) { g.b = g.a; g.ldb = g.lda; g.J = g.I; g.o.y = nullptr; }      // one column of tiles, whose products nobody reads
     const Out o = g.o;
     g.tiles_j = out ? (int)p.tiles_j : 1;
@@ -814,10 +825,11 @@ int product(const Plan &p, TileArgs g, float *part, float *sums, int parts, T *s
     g.slices = p.slices;
     g.sums = sums_out && !parts ? sums : nullptr;
     g.sums_out = p.slices == 1 ? sums_out : nullptr;
-    if (p.slices > 1 && out) g.o.part = part;
+    const int slices = p.slices * (g.low ? 2 : 1);
+    if (slices > 1 && out) g.o.part = part;
     if (launch_tile<T, AC, BC>(p, g, st)) return 1;
-    if (p.slices == 1 && !parts) return 0;
-    return join<T>(p, g, o, p.slices > 1 && out ? part : nullptr, sums, parts ? parts : p.slices, sums_out, st);
+    if (slices == 1 && !parts) return 0;
+    return join<T>(slices, g, o, slices > 1 && out ? part : nullptr, sums, parts ? parts : slices, sums_out, st);
 }
 
 // dz is formed once, rounded to the type, ahead of both products.  Formed in their loads instead (dy times the slopes, two
@@ -825,6 +837,15 @@ int product(const Plan &p, TileArgs g, float *part, float *sums, int parts, T *s
 // types would read both once per column of tiles.  Where dz is rounded, the pass that forms it adds up the bias gradient
 // from the unrounded values; elsewhere dW's tiles add up the columns they read anyway.
 struct DzPlan { int lanes, parts; int64_t blocks_x, rows; };
+
+// Rounding dz adds an error of the size of the result's own rounding.  Over many values that is their root mean square;
+// where few values of dz, or few results, carry all of it, chance can make it the larger part.  There the products are
+// short, and dz goes in as two rounded parts, as slices of one reduction: its error is then that of float32 sums.
+// (9689 x 83 x 5 backward with silu in bfloat16: 46.7 us, in one part 41.1 with dW 1.5 times as far off as a rounded exact
+// result.)  I, J: of the product; other: values of its second operand.
+bool two_parts(int64_t M, int64_t N, int64_t I, int64_t J, int64_t other, int dtype, int act) {
+    return dtype != kF32 && act != ACT_NONE && act != ACT_RELU && std::min(M * N, I * J) <= 4096 && I * J <= (1 << 19) && other <= (1 << 22);
+}
 DzPlan dz_plan(int64_t M, int64_t N, int dtype, int act) {
     DzPlan d = {};
     if (dtype == kF32 || act == ACT_NONE || act == ACT_RELU || M == 0 || N == 0) return d;
@@ -842,9 +863,10 @@ struct BwdWs { int64_t sums, part, bytes; };
 BwdWs bwd_ws(int64_t M, int64_t K, int64_t N, int dtype, int act) {
     BwdWs w;
     const Plan dx = plan(M, K, N, dtype), dw = plan(N, K, M, dtype);
-    w.sums = act == ACT_NONE ? 0 : up256(M * N * elem_size(dtype));
+    const bool low_x = two_parts(M, N, M, K, N * K, dtype, act), low_w = two_parts(M, N, N, K, M * K, dtype, act);
+    w.sums = act == ACT_NONE ? 0 : up256((low_x || low_w ? 2 : 1) * M * N * elem_size(dtype));
     w.part = w.sums + up256((int64_t)std::max(dw.slices, dz_plan(M, N, dtype, act).parts) * N * 4);
-    w.bytes = w.part + std::max(dx.ws, dw.ws);
+    w.bytes = w.part + std::max(low_x ? up256(2 * dx.slices * M * K * 4) : dx.ws, low_w ? up256(2 * dw.slices * N * K * 4) : dw.ws);
     return w;
 }
 
@@ -906,15 +928,25 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
     const T *dz = dy;
     int64_t lddz = lddy;
     DzPlan d = {};
+    const bool low_x = dx && two_parts(M, N, M, K, N * K, dtype, act), low_w = dw && two_parts(M, N, N, K, M * K, dtype, act);
+    const int64_t low = low_x || low_w ? M * N : 0;
     if (act != ACT_NONE && M > 0 && N > 0 && (dx || dw || db)) {
         T *z = (T *)ws;
         constexpr int E = Elem<T>::per_chunk;
         const unsigned blocks = (unsigned)std::min<int64_t>((M * ((N + E - 1) / E) + 255) / 256, 256 * 32);
         if (db) d = dz_plan(M, N, dtype, act);
+        auto form = [&](auto a, auto l) {
+            constexpr int ACT = decltype(a)::value;
+            constexpr bool LOW = decltype(l)::value;
+            if (d.parts) hipLaunchKernelGGL((k_dz_sums<T, ACT, LOW>), dim3((unsigned)d.blocks_x, (unsigned)d.parts), dim3(256), 0, st, dy, lddy, kept,
+                                            ldk, z, low, M, N, d.lanes, d.rows, sums);
+            else hipLaunchKernelGGL((k_dz<T, ACT, LOW>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, low, M, N);
+        };
         with_act(act, [&](auto a) {
-            if (d.parts) hipLaunchKernelGGL((k_dz_sums<T, decltype(a)::value>), dim3((unsigned)d.blocks_x, (unsigned)d.parts), dim3(256), 0, st, dy, lddy,
-                                            kept, ldk, z, M, N, d.lanes, d.rows, sums);
-            else hipLaunchKernelGGL((k_dz<T, decltype(a)::value>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, M, N);
+            if constexpr (sizeof(T) == 2) {
+                if (low) return form(a, std::true_type{});
+            }
+            form(a, std::false_type{});
         });
         CAFE_HIP_CHECK(hipGetLastError());
         dz = z; lddz = N;
@@ -924,12 +956,14 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
     if (dx) {
         TileArgs q = g;
         q.b = w; q.ldb = ldw; q.I = M; q.J = K; q.R = N;
+        q.low = low_x ? low : 0;
         q.o.y = dx; q.o.ldy = lddx;
         if (product<T, false, true>(plan(M, K, N, dtype), q, part, nullptr, 0, nullptr, st)) return 1;
     }
     if (dw || db) {
         TileArgs q = g;
         q.b = x; q.ldb = ldx; q.I = N; q.J = K; q.R = M;
+        q.low = low_w ? low : 0;
         q.o.y = dw; q.o.ldy = K;
         return product<T, true, true>(plan(N, K, M, dtype), q, part, sums, d.parts, db, st);
     }

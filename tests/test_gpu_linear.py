@@ -369,3 +369,20 @@ def test_the_bias_gradient_alone(t, act):
         want = linear_backward(dy, x, w, kept, act)
         db = linear_backward(dy, x, w, kept, act, need=(False, False, True))
         assert db[0] is None and db[1] is None and torch.equal(db[2], want[2])
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(9689, 83, 5), (16, 300, 200), (1, 40, 3), (900, 7, 4)])
+def test_few_results_are_rounded_once(m, k, n, t):
+    """Where min(values of dz, results) is at most 4096, dz enters the products in two parts: what is left of its rounding
+    is half a step of half a step, the rounding of the result stands alone."""
+    x, w, _, _, dy = make(m, k, n, t)
+    s = torch.rand(m, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) + 0.5
+    dx, dw, _ = linear_backward(dy, x, w, Slope(s), "silu")
+    dz, xd, wd = dy.double() * s.double(), x.double(), w.double()
+    h = half_step(t) ** 2 * 1.02 + U32                      # of a value of dz; below float16's normal range half a subnormal step
+    low = tiny(t)
+    for got, want, mag, other, terms in ((dx, dz @ wd, dz.abs() @ wd.abs(), torch.ones_like(dz) @ wd.abs(), n),
+                                         (dw, dz.t() @ xd, dz.t().abs() @ xd.abs(), torch.ones_like(dz).t() @ xd.abs(), m)):
+        if min(m * n, want.numel()) <= 4096:
+            check(got, want, (h + (2 * 2 * terms + 16) * U32) * mag + low * other + half_step(t) * 1.01 * want.abs() + tiny(t), "product")
