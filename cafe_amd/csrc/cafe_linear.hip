@@ -102,7 +102,7 @@ struct Out {
 struct TileArgs {
     const void *a, *b;
     int64_t lda, ldb;
-    int64_t low;                      // != 0: A stands for A + what lies that many elements behind it
+    int64_t low;                      // != 0: A is the sum of two matrices, the second that many elements behind the first
     int64_t I, J, R;                  // C is [I, J], the reduction runs over R
     float *sums; void *sums_out;      // column sums of A: per slice, or (one slice) the result itself; null: not wanted
     int tiles_j, tiles;               // tiles along j, tiles in all
@@ -144,7 +144,8 @@ template <class T, int TI, int TJ> __device__ __forceinline__ void mfma_step(con
 // A lane's fragment for step s holds the reductions 2s+h (h = lane / 32) chunk of 16 bytes in both layouts.
 // What lies outside the operand reads as 0; nothing outside is touched: a chunk that would cross a row's end is read
 // further back and shifted.
-template <class T, bool COLS, int BX, int THREADS> struct Operand {
+// PARTS 2: the operand is the sum of two matrices, BX / 2 entries of the first and the same of the second, `low` elements on.
+template <class T, bool COLS, int PARTS, int BX, int THREADS> struct Operand {
     static constexpr int E = Elem<T>::per_chunk;
     static constexpr int BK = 8 * E;
     static constexpr int CPR = COLS ? BX / E : 8;                          // 16-byte chunks per LDS row
@@ -162,12 +163,17 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
     int64_t R, X, ld, x0;
     const T *base;
 
-    __device__ __forceinline__ void init(const void *src, int64_t ld_, int64_t X_, int64_t R_, int64_t x0_) {
+    static constexpr int ENTRIES = BX / PARTS;                             // rows i or j of the tile
+    static_assert(ENTRIES % E == 0, "");
+
+    __device__ __forceinline__ static int column() { return threadIdx.x % CPR * E % ENTRIES; }      // columns: of the thread's chunk
+    __device__ __forceinline__ void init(const void *src, int64_t ld_, int64_t X_, int64_t R_, int64_t x0_, int64_t low = 0) {
         base = (const T *)src; ld = ld_; X = X_; R = R_; x0 = x0_;
         const int t = threadIdx.x, c = t % CPR, row = t / CPR;
         if (COLS) {
+            if (PARTS > 1 && c * E >= ENTRIES) base += low;
             tiny = X < E;
-            int64_t col = x0 + c * E, start = col + E > X ? X - E : col;
+            int64_t col = x0 + column(), start = col + E > X ? X - E : col;
             if (tiny) start = 0;
             shift = (int)(col - start > E ? E : col - start);
             adv = BK * ld;
@@ -179,13 +185,14 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
             adv = BK;
 #pragma unroll
             for (int n = 0; n < N; n++) {
-                int64_t i = x0 + row + n * STEP;
+                const int e = row + n * STEP;
+                int64_t i = x0 + e % ENTRIES;
                 if (i >= X) i = X - 1;                                     // rows behind the last one repeat it; never stored
-                p[n] = base + i * ld + c * E;
+                p[n] = base + i * ld + c * E + (PARTS > 1 && e >= ENTRIES ? low : 0);
             }
         }
     }
-    __device__ __forceinline__ bool edge() const { return COLS && x0 + BX > X; }       // columns end inside this tile
+    __device__ __forceinline__ bool edge() const { return COLS && x0 + ENTRIES > X; }       // columns end inside this tile
     // Requests tile kt, which lies inside the operand.
     __device__ __forceinline__ void load_inner(u32x4 (&reg)[N], int64_t kt) const {
 #pragma unroll
@@ -200,7 +207,7 @@ template <class T, bool COLS, int BX, int THREADS> struct Operand {
 #pragma unroll
             for (int n = 0; n < N; n++) {
                 const int64_t r = row + n * STEP;
-                if (COLS) reg[n] = kt * BK + r < R ? load_some(base + (kt * BK + r) * ld + x0 + c * E, (int)(X - x0 - c * E)) : u32x4{0, 0, 0, 0};
+                if (COLS) reg[n] = kt * BK + r < R ? load_some(base + (kt * BK + r) * ld + x0 + column(), (int)(X - x0 - column())) : u32x4{0, 0, 0, 0};
                 else { const int64_t k = kt * BK + c * E; reg[n] = k < R ? load_some(p[n] + kt * BK, (int)(R - k)) : u32x4{0, 0, 0, 0}; }
             }
         } else if (COLS) {
@@ -304,19 +311,22 @@ template <int MF, int R, int W, int V> __device__ __forceinline__ void weave() {
 // library product reaches 153) and 1010 TF in bfloat16 (136 us; 1341), 8192 x 1024 x 1024 at 120-126 and 716.  Short
 // reductions are bound by what surrounds the products, filling the pipeline and passing the tile through LDS: dx at
 // 16384 x 3341 with a reduction of 256 takes 70 us in bfloat16, 1.6 TB/s of stores (66 with rows on 16-byte boundaries).
-template <class T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
+//
+// PARTS 2: A is the sum of two matrices (dz's rounded values and what their rounding left).  The tile's BM entries are
+// BM / 2 rows of both, so that both meet the same B in LDS, and their products are added on the way out.  16384 x 3341 x 256
+// in bfloat16, forward and backward, takes 283 us (with one part 215; with the parts one behind the other along the
+// reduction 341, registers spilled).
+template <class T, bool ACOLS, bool BCOLS, int PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
     constexpr int TH = WM * WN * 64, TI = BM / WM / 32, TJ = BN / WN / 32, E = Elem<T>::per_chunk, PF = sizeof(T) == 4 ? 1 : 2;
-    typedef Operand<T, ACOLS, BM, TH> OA;
-    typedef Operand<T, BCOLS, BN, TH> OB;
-    constexpr int BK = OA::BK, STAGE = OA::BYTES + OB::BYTES, CS = BN + 8;
+    typedef Operand<T, ACOLS, PARTS, BM, TH> OA;
+    typedef Operand<T, BCOLS, 1, BN, TH> OB;
+    constexpr int BK = OA::BK, ROWS = BM / PARTS, STAGE = OA::BYTES + OB::BYTES, CS = BN + 8;
     __shared__ __align__(16) char lds[2 * STAGE > BM * CS * 4 ? 2 * STAGE : BM * CS * 4];
     const int tile = xcd_tile(blockIdx.x, g.tiles);
-    const int64_t i0 = (int64_t)(tile / g.tiles_j) * BM, j0 = (int64_t)(tile % g.tiles_j) * BN;
+    const int64_t i0 = (int64_t)(tile / g.tiles_j) * ROWS, j0 = (int64_t)(tile % g.tiles_j) * BN;
     const int64_t kts = (g.R + BK - 1) / BK;
-    const bool second = (int)blockIdx.y >= g.slices;                       // slices of A's second part (g.low), over the same B
-    const int slice = blockIdx.y - (second ? g.slices : 0);
-    const int64_t k0 = kts * slice / g.slices, k1 = kts * (slice + 1) / g.slices;
+    const int64_t k0 = kts * blockIdx.y / g.slices, k1 = kts * (blockIdx.y + 1) / g.slices;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
     f32x16 acc[TI][TJ];
@@ -328,10 +338,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             for (int e = 0; e < 16; e++) acc[a][b][e] = 0.f;
     OA A;
     OB B;
-    A.init((const T *)g.a + (second ? g.low : 0), g.lda, g.I, g.R, i0);
+    A.init(g.a, g.lda, g.I, g.R, i0, g.low);
     B.init(g.b, g.ldb, g.J, g.R, j0);
     u32x4 ra[PF][OA::N], rb[PF][OB::N];
-    const bool sums = ACOLS && BCOLS && g.sums && j0 == 0;
+    const bool sums = ACOLS && BCOLS && PARTS == 1 && g.sums && j0 == 0;
     float cs[E];
 #pragma unroll
     for (int e = 0; e < E; e++) cs[e] = 0.f;
@@ -424,7 +434,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
         };
         if (k0 + 2 * PF >= inner) start(std::integral_constant<int, 0>{});
         else if (woven && !sums) run(std::integral_constant<int, 2>{});
-        else if constexpr (ACOLS && BCOLS) {
+        else if constexpr (ACOLS && BCOLS && PARTS == 1) {
             constexpr int WITH_SUMS = BM < 256 ? 3 : 1;             // 3 would spill registers in the largest tile
             if (woven) run(std::integral_constant<int, WITH_SUMS>{});
             else run(std::integral_constant<int, 1>{});
@@ -460,7 +470,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             for (int e = 0; e < 16; e++)
                 c[(wi + 32 * a + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * CS + wj + 32 * b + (lane & 31)] = acc[a][b][e];
     __syncthreads();
-    constexpr int CH = BN / E, PASS = BM * CH / TH;
+    constexpr int CH = BN / E, PASS = ROWS * CH / TH;
+    static_assert(ROWS * CH % TH == 0, "");
     const int col = threadIdx.x % CH * E;
     const int64_t j = j0 + col;
     const int left = (int)(g.J - j < E ? g.J - j : E);
@@ -473,7 +484,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             const int64_t i = i0 + row;
             if (i >= g.I) break;
 #pragma unroll
-            for (int h = 0; h < E; h += 4) store_some(part + i * g.J + j + h, *(const u32x4 *)(c + row * CS + col + h), left - h);
+            for (int h = 0; h < E; h += 4) {
+                f32x4 v = *(const f32x4 *)(c + row * CS + col + h);
+                if constexpr (PARTS > 1) v += *(const f32x4 *)(c + (row + ROWS) * CS + col + h);
+                store_some(part + i * g.J + j + h, __builtin_bit_cast(u32x4, v), left - h);
+            }
         }
         return;
     }
@@ -487,7 +502,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_tile(TileArgs g) {
             if (i >= g.I) break;
             float v[E];
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = c[row * CS + col + e];
+            for (int e = 0; e < E; e++) v[e] = PARTS > 1 ? c[row * CS + col + e] + c[(row + ROWS) * CS + col + e] : c[row * CS + col + e];
             finish<T, decltype(actc)::value>(g.o, i, j, v, bias, left);
         }
     };
@@ -648,11 +663,16 @@ template <class T, int FT, int WAVES, bool MANY_W> __global__ __launch_bounds__(
     }
 }
 
-// dz = dy * act'(z), rounded.  kept: z in the type (relu: anything of its sign), or the slopes in float32.  One 16-byte
-// chunk per thread and step.  SUMS: the column sums of the unrounded values over the block's rows, a row of `sums` per
-// blockIdx.y; a block then has `lanes` chunks side by side.  LOW: what the rounding left, rounded, `low` values further.  Bound by memory: 8192 x 1024 in float32 takes 15.3 us (6.5
-// TB/s, cached in part), 16384 x 256 in bfloat16 with float32 slopes and sums 10.2 (3.3 TB/s; 7 without the sums).
-template <class T, int ACT, bool LOW> __device__ __forceinline__ void dz_chunk(const T *dy, const void *kept, int64_t at_kept, T *dz, int64_t low, int left, float *g) {
+// Whether dz = dy act'(z) of type T is held as two rounded parts: the rounded value, and what the rounding left, rounded.
+// Both products take both parts, so that dx and dW carry one rounding, their own (with one part they were 1.4 times as far
+// from the exact gradients as those rounded once).  relu and no activation leave dy's own values, which need no rounding.
+template <class T, int ACT> constexpr bool two_parts = sizeof(T) == 2 && ACT != ACT_NONE && ACT != ACT_RELU;
+
+// dz = dy * act'(z), rounded; of two parts: what the rounding left, rounded, `low` values further.  kept: z in the type (relu:
+// anything of its sign), or the slopes in float32.  One 16-byte chunk per thread and step.  k_dz_sums: and the column sums of
+// the unrounded values over the block's rows, a row of `sums` per blockIdx.y; a block has `lanes` chunks side by side.
+// Bound by memory: 8192 x 1024 in float32 takes 15.3 us (6.5 TB/s, cached in part).
+template <class T, int ACT> __device__ __forceinline__ void dz_chunk(const T *dy, const void *kept, int64_t at_kept, T *dz, int64_t low, int left, float *g) {
     constexpr int E = Elem<T>::per_chunk;
     float k[E];
     unpack<T>(load_some(dy, left), g);
@@ -666,7 +686,7 @@ template <class T, int ACT, bool LOW> __device__ __forceinline__ void dz_chunk(c
     for (int e = 0; e < E; e++) g[e] = through<ACT>(g[e], k[e]);
     const u32x4 high = pack<T>(g);
     store_some(dz, high, left);
-    if constexpr (LOW) {
+    if constexpr (two_parts<T, ACT>) {
         float h[E];
         unpack<T>(high, h);
 #pragma unroll
@@ -674,17 +694,17 @@ template <class T, int ACT, bool LOW> __device__ __forceinline__ void dz_chunk(c
         store_some(dz + low, pack<T>(h), left);
     }
 }
-template <class T, int ACT, bool LOW>
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_dz(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t low, int64_t M, int64_t N) {
     constexpr int E = Elem<T>::per_chunk;
     const int64_t chunks = (N + E - 1) / E, n = M * chunks;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < n; q += (int64_t)gridDim.x * 256) {
         const int64_t m = q / chunks, col = (q - m * chunks) * E;
         float g[E];
-        dz_chunk<T, ACT, LOW>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, (int)(N - col < E ? N - col : E), g);
+        dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, (int)(N - col < E ? N - col : E), g);
     }
 }
-template <class T, int ACT, bool LOW>
+template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const void *kept, int64_t ldk, T *dz, int64_t low, int64_t M, int64_t N,
                                                 int lanes, int64_t rows, float *sums) {
     constexpr int E = Elem<T>::per_chunk;
@@ -699,7 +719,7 @@ __global__ __launch_bounds__(256) void k_dz_sums(const T *dy, int64_t ldy, const
 #pragma unroll 4
         for (int64_t m = blockIdx.y * rows + y; m < m1; m += ny) {
             float g[E];
-            dz_chunk<T, ACT, LOW>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, left, g);
+            dz_chunk<T, ACT>(dy + m * ldy + col, kept, m * ldk + col, dz + m * N + col, low, left, g);
 #pragma unroll
             for (int e = 0; e < E; e++) s[e] += g[e];
         }
@@ -738,7 +758,8 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 struct Plan { int bm, bn; int64_t tiles_i, tiles_j, tiles; int slices; int64_t ws; double us; };
 struct Cost { double shared[4], alone[4], ends, join, per_slice, launch; };
 
-Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
+// parts: of the first operand (2: a tile holds half as many of its rows).
+Plan plan(int64_t I, int64_t J, int64_t R, int dtype, int parts = 1) {
     static const Cost f32 = {{0, 1.85, 1.01, 0.54}, {0, 2.25, 1.25, 0.68}, 2.4, 1.8, 0.05, 4.8};
     static const Cost half = {{0.92, 0.665, 0.49, 0.27}, {0.98, 0.665, 0.49, 0.293}, 1.25, 2.5, 0.13, 4.55};
     static const struct { int bm, bn, kind; } tiles[] = {{256, 128, 0}, {128, 128, 1}, {128, 64, 2}, {64, 128, 2}, {64, 64, 3}};
@@ -747,7 +768,7 @@ Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
     Plan best = {};
     for (const auto &t : tiles) {
         if (t.kind == 0 && dtype == kF32) continue;
-        const int64_t ti = (I + t.bm - 1) / t.bm, tj = std::max<int64_t>(1, (J + t.bn - 1) / t.bn);
+        const int64_t ti = (I + t.bm / parts - 1) / (t.bm / parts), tj = std::max<int64_t>(1, (J + t.bn - 1) / t.bn);
         for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64}) {
             if (s > 1 && (ti * tj * s > 2048 || kts < 2 * s)) break;
             const double load = std::ceil((double)ti * tj * s / 256.0), steps = (double)((kts + s - 1) / s);
@@ -760,15 +781,15 @@ Plan plan(int64_t I, int64_t J, int64_t R, int dtype) {
     return best;
 }
 
-template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, hipStream_t st) {
+template <class T, bool AC, bool BC, int P> int launch_tile_of(const Plan &p, TileArgs g, hipStream_t st) {
     if (p.tiles > (int64_t)1 << 22) {                       // a grid holds fewer than 2^32 work items; INT32_MAX tiles are far behind it
         set_error("cafe_linear: %lld tiles of %d x %d are more than a launch takes", (long long)p.tiles, p.bm, p.bn);
         return 1;
     }
-    const dim3 grid((unsigned)g.tiles, (unsigned)(p.slices * (g.low ? 2 : 1)));
+    const dim3 grid((unsigned)g.tiles, (unsigned)p.slices);
     if constexpr (sizeof(T) == 2) {
         if (p.bm == 256) {
-            hipLaunchKernelGGL((k_tile<T, AC, BC, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
+            hipLaunchKernelGGL((k_tile<T, AC, BC, P, 256, 128, 4, 2>), grid, dim3(512), 0, st, g);
             CAFE_HIP_CHECK(hipGetLastError());
             return 0;
         }
@@ -777,12 +798,19 @@ template <class T, bool AC, bool BC> int launch_tile(const Plan &p, TileArgs g, 
     // too short to cover a wave's own waits, a second wave on the unit does (16384 x 3341 x 256 in bfloat16 47.8 us, with
     // four waves 51.3; 8192 x 1024 outputs over 479 across rows 15.9 and 19.6).  float32 with eight waves loses 4-10 % in dx.
     constexpr int W = sizeof(T) == 2 ? 2 : 1;
-    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 128, 64, 2 * W, 2>), grid, dim3(256 * W), 0, st, g);
-    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
-    else hipLaunchKernelGGL((k_tile<T, AC, BC, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
+    if (p.bm == 128 && p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, P, 128, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, P, 128, 64, 2 * W, 2>), grid, dim3(256 * W), 0, st, g);
+    else if (p.bn == 128) hipLaunchKernelGGL((k_tile<T, AC, BC, P, 64, 128, 2, 2 * W>), grid, dim3(256 * W), 0, st, g);
+    else hipLaunchKernelGGL((k_tile<T, AC, BC, P, 64, 64, 2, 2>), grid, dim3(256), 0, st, g);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
+}
+
+template <class T, bool AC, bool BC> int launch_tile(const Plan &p, const TileArgs &g, hipStream_t st) {
+    if constexpr (sizeof(T) == 2 && BC) {
+        if (g.low) return launch_tile_of<T, AC, BC, 2>(p, g, st);
+    }
+    return launch_tile_of<T, AC, BC, 1>(p, g, st);
 }
 
 template <class F> void with_act(int act, F f) {
@@ -825,30 +853,21 @@ int product(const Plan &p, TileArgs g, float *part, float *sums, int parts, T *s
     g.slices = p.slices;
     g.sums = sums_out && !parts ? sums : nullptr;
     g.sums_out = p.slices == 1 ? sums_out : nullptr;
-    const int slices = p.slices * (g.low ? 2 : 1);
-    if (slices > 1 && out) g.o.part = part;
+    if (p.slices > 1 && out) g.o.part = part;
     if (launch_tile<T, AC, BC>(p, g, st)) return 1;
-    if (slices == 1 && !parts) return 0;
-    return join<T>(slices, g, o, slices > 1 && out ? part : nullptr, sums, parts ? parts : slices, sums_out, st);
+    if (p.slices == 1 && !parts) return 0;
+    return join<T>(p.slices, g, o, p.slices > 1 && out ? part : nullptr, sums, parts ? parts : p.slices, sums_out, st);
 }
 
-// dz is formed once, rounded to the type, ahead of both products.  Formed in their loads instead (dy times the slopes, two
-// operands read in place of one) it cost float32 more than it saved: 321 us against 307 at 8192 x 1024 x 1024; 16-bit
-// types would read both once per column of tiles.  Where dz is rounded, the pass that forms it adds up the bias gradient
-// from the unrounded values; elsewhere dW's tiles add up the columns they read anyway.
+// dz is formed once, ahead of both products.  Formed in their loads instead (dy times the slopes, two operands read in place
+// of one) it cost float32 more than it saved: 321 us against 307 at 8192 x 1024 x 1024; 16-bit types would read both once
+// per column of tiles.  Where dz is rounded, the pass that forms it adds up the bias gradient from the unrounded values;
+// elsewhere dW's tiles add up the columns they read anyway.
 struct DzPlan { int lanes, parts; int64_t blocks_x, rows; };
-
-// Rounding dz adds an error of the size of the result's own rounding.  Over many values that is their root mean square;
-// where few values of dz, or few results, carry all of it, chance can make it the larger part.  There the products are
-// short, and dz goes in as two rounded parts, as slices of one reduction: its error is then that of float32 sums.
-// (9689 x 83 x 5 backward with silu in bfloat16: 46.7 us, in one part 41.1 with dW 1.5 times as far off as a rounded exact
-// result.)  I, J: of the product; other: values of its second operand.
-bool two_parts(int64_t M, int64_t N, int64_t I, int64_t J, int64_t other, int dtype, int act) {
-    return dtype != kF32 && act != ACT_NONE && act != ACT_RELU && std::min(M * N, I * J) <= 4096 && I * J <= (1 << 19) && other <= (1 << 22);
-}
+int dz_parts(int dtype, int act) { return dtype != kF32 && act != ACT_NONE && act != ACT_RELU ? 2 : 1; }
 DzPlan dz_plan(int64_t M, int64_t N, int dtype, int act) {
     DzPlan d = {};
-    if (dtype == kF32 || act == ACT_NONE || act == ACT_RELU || M == 0 || N == 0) return d;
+    if (dz_parts(dtype, act) == 1 || M == 0 || N == 0) return d;
     const int64_t chunks = (N + 7) / 8;
     for (d.lanes = 1; d.lanes < 64 && d.lanes < chunks;) d.lanes *= 2;
     d.blocks_x = (chunks + d.lanes - 1) / d.lanes;
@@ -862,11 +881,11 @@ DzPlan dz_plan(int64_t M, int64_t N, int dtype, int act) {
 struct BwdWs { int64_t sums, part, bytes; };
 BwdWs bwd_ws(int64_t M, int64_t K, int64_t N, int dtype, int act) {
     BwdWs w;
-    const Plan dx = plan(M, K, N, dtype), dw = plan(N, K, M, dtype);
-    const bool low_x = two_parts(M, N, M, K, N * K, dtype, act), low_w = two_parts(M, N, N, K, M * K, dtype, act);
-    w.sums = act == ACT_NONE ? 0 : up256((low_x || low_w ? 2 : 1) * M * N * elem_size(dtype));
+    const int parts = dz_parts(dtype, act);
+    const Plan dx = plan(M, K, N, dtype, parts), dw = plan(N, K, M, dtype, parts);
+    w.sums = act == ACT_NONE ? 0 : up256(parts * M * N * elem_size(dtype));
     w.part = w.sums + up256((int64_t)std::max(dw.slices, dz_plan(M, N, dtype, act).parts) * N * 4);
-    w.bytes = w.part + std::max(low_x ? up256(2 * dx.slices * M * K * 4) : dx.ws, low_w ? up256(2 * dw.slices * N * K * 4) : dw.ws);
+    w.bytes = w.part + std::max(dx.ws, dw.ws);
     return w;
 }
 
@@ -928,44 +947,35 @@ int bwd(const T *dy, int64_t lddy, const T *x, int64_t ldx, const T *w, int64_t 
     const T *dz = dy;
     int64_t lddz = lddy;
     DzPlan d = {};
-    const bool low_x = dx && two_parts(M, N, M, K, N * K, dtype, act), low_w = dw && two_parts(M, N, N, K, M * K, dtype, act);
-    const int64_t low = low_x || low_w ? M * N : 0;
+    const int parts = dz_parts(dtype, act);
+    const int64_t low = parts == 2 ? M * N : 0;
     if (act != ACT_NONE && M > 0 && N > 0 && (dx || dw || db)) {
         T *z = (T *)ws;
         constexpr int E = Elem<T>::per_chunk;
         const unsigned blocks = (unsigned)std::min<int64_t>((M * ((N + E - 1) / E) + 255) / 256, 256 * 32);
         if (db) d = dz_plan(M, N, dtype, act);
-        auto form = [&](auto a, auto l) {
-            constexpr int ACT = decltype(a)::value;
-            constexpr bool LOW = decltype(l)::value;
-            if (d.parts) hipLaunchKernelGGL((k_dz_sums<T, ACT, LOW>), dim3((unsigned)d.blocks_x, (unsigned)d.parts), dim3(256), 0, st, dy, lddy, kept,
-                                            ldk, z, low, M, N, d.lanes, d.rows, sums);
-            else hipLaunchKernelGGL((k_dz<T, ACT, LOW>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, low, M, N);
-        };
         with_act(act, [&](auto a) {
-            if constexpr (sizeof(T) == 2) {
-                if (low) return form(a, std::true_type{});
-            }
-            form(a, std::false_type{});
+            constexpr int ACT = decltype(a)::value;
+            if (d.parts) hipLaunchKernelGGL((k_dz_sums<T, ACT>), dim3((unsigned)d.blocks_x, (unsigned)d.parts), dim3(256), 0, st, dy, lddy, kept,
+                                            ldk, z, low, M, N, d.lanes, d.rows, sums);
+            else hipLaunchKernelGGL((k_dz<T, ACT>), dim3(blocks), dim3(256), 0, st, dy, lddy, kept, ldk, z, low, M, N);
         });
         CAFE_HIP_CHECK(hipGetLastError());
         dz = z; lddz = N;
     }
     TileArgs g = {};
-    g.a = dz; g.lda = lddz;
+    g.a = dz; g.lda = lddz; g.low = low;
     if (dx) {
         TileArgs q = g;
         q.b = w; q.ldb = ldw; q.I = M; q.J = K; q.R = N;
-        q.low = low_x ? low : 0;
         q.o.y = dx; q.o.ldy = lddx;
-        if (product<T, false, true>(plan(M, K, N, dtype), q, part, nullptr, 0, nullptr, st)) return 1;
+        if (product<T, false, true>(plan(M, K, N, dtype, parts), q, part, nullptr, 0, nullptr, st)) return 1;
     }
     if (dw || db) {
         TileArgs q = g;
         q.b = x; q.ldb = ldx; q.I = N; q.J = K; q.R = M;
-        q.low = low_w ? low : 0;
         q.o.y = dw; q.o.ldy = K;
-        return product<T, true, true>(plan(N, K, M, dtype), q, part, sums, d.parts, db, st);
+        return product<T, true, true>(plan(N, K, M, dtype, parts), q, part, sums, d.parts, db, st);
     }
     return 0;
 }
