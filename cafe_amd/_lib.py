@@ -96,6 +96,8 @@ SYMBOLS = {
     "cafe_interact_bwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64] + [ctypes.c_int] * 5
                               + [_vp, _i64, _vp, _i64, _i64, _vp]),
     "cafe_adamw_dev": (ctypes.c_int, [_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
+    "cafe_adamw_dither_dev": (ctypes.c_int, [_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 5
+                              + [_i64, _vp, _i64, _vp, _vp]),
     "cafe_adamw_tick_dev": (ctypes.c_int, [_vp, _vp] + [ctypes.c_double] * 4 + [_vp, _vp]),
     "cafe_moment8_values_dev": (ctypes.c_int, [_i64p, ctypes.c_int, _vp]),
     "cafe_grad_norm_dev": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]),

@@ -51,7 +51,7 @@ def _check_moments8(moments, counts, index, what):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-               masters=None, factors=None):
+               masters=None, factors=None, dither=None):
     """One AdamW step in place over lists of tensors:
 
         m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
@@ -62,7 +62,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     None, or float32 tensors of the parameters' shapes that are updated in their place; the parameters then receive the
     rounded values (a float32 parameter may be its own master).  step: the number of this step, from 1; it is a number of
     the host, so a call under graph capture takes `factors` instead (adamw_tick), a float32 tensor of three on the device.
-    All arithmetic is float32."""
+    dither: for Moment8, the number of this step in a run of them, from 1, or an int64 tensor of one on the device (under
+    capture: the tensor that adamw_tick counts in); AdamW always gives it.  From the ninth step on the moments are rounded up
+    or down with the probabilities that leave their mean in place, by a hash of this number and a value's index.  Without it
+    they are rounded to nearest: right for a single step, but in a run of them v would stand still, since a step changes it by
+    less than half a code.  All arithmetic is float32."""
     n = len(params)
     if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n) or (masters is not None and len(masters) != n):
         raise ValueError("params, grads, moments and masters are lists of one length")
@@ -97,6 +101,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     written += [a for a, p, c in zip(cols[6], cols[0], counts) if c and a and a != p]
     if len(set(written)) != len(written):
         raise ValueError("a parameter, moment or master is listed twice")
+    count = None
+    if isinstance(dither, torch.Tensor):
+        _check([dither], torch.int64, index, [1], "dither")
+        count, dither = dither.data_ptr(), 0
+    elif dither is None:
+        dither = 0
+    elif int(dither) != dither or dither < 1:
+        raise ValueError(f"dither {dither}: the number of this step, from 1")
     on_device(first)
     if factors is None:
         if step is None or int(step) != step or step < 1:
@@ -107,11 +119,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step=None, lr, betas=(0.
     else:
         _check([factors], torch.float32, index, [3], "factors")
         step = 0
+    if eight and dither and torch.cuda.is_current_stream_capturing():
+        raise _lib.CafeError("a captured step would repeat the same random bits: give `dither` as a tensor")
     flat = (ctypes.c_int64 * (8 * n))(*[a for c in cols for a in c])
     with launch_on(first) as st:
-        _lib.check(_lib.load().cafe_adamw_dev(flat, n, DTYPE_CODE[dtype], 8 if eight else 32, float(lr), float(betas[0]), float(betas[1]),
-                                              float(eps), float(weight_decay), step, None if factors is None else factors.data_ptr(), st),
-                   "cafe_adamw_dev")
+        _lib.check(_lib.load().cafe_adamw_dither_dev(flat, n, DTYPE_CODE[dtype], 8 if eight else 32, float(lr), float(betas[0]),
+                                                     float(betas[1]), float(eps), float(weight_decay), step,
+                                                     None if factors is None else factors.data_ptr(), int(dither), count, st),
+                   "cafe_adamw_dither_dev")
     torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])     # a backward that kept one says so
 
 
@@ -156,7 +171,8 @@ def moment8_values(exp_avgs, exp_avg_sqs):
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update in one launch per type and step count.
 
-    state_bits: 32, or 8 for moments of one byte per value (plus one per 256).  master_weights: bfloat16 and float16
+    state_bits: 32, or 8 for moments of one byte per value (plus one per 256): right on average, each within some 20 % (their
+    rounding is random, by a hash that repeats from run to run).  master_weights: bfloat16 and float16
     parameters keep a float32 copy that the steps accumulate in (default True; ignored for float32).  capturable: the
     step count of a parameter group lives on the device, so that step() can be captured into a graph and replayed; lr may
     then be a float32 tensor of one element on the device, and parameters without a gradient are skipped but do not lag
@@ -217,11 +233,11 @@ class AdamW(torch.optim.Optimizer):
                 sets.setdefault(key, []).append((p, st))
             ticked = {}
             for (device, _, step, _, master), members in sets.items():
-                kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step)
+                kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step, dither=step)
                 if group["capturable"]:
                     if device not in ticked:
                         ticked[device] = self._tick(group, device)
-                    kw.update(step=None, lr=0.0, factors=ticked[device])
+                    kw.update(step=None, lr=0.0, factors=ticked[device][1], dither=ticked[device][0])
                 moments = [self._moments(st) for _, st in members]
                 adamw_step([p for p, _ in members], [p.grad for p, _ in members], [m for m, _ in moments], [v for _, v in moments],
                            masters=[st["master"] for _, st in members] if master else None, **kw)
@@ -229,7 +245,7 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _tick(group, device):
-        """The group's device-side count on `device`, advanced, and its factors."""
+        """(count, factors): the group's device-side step count on `device`, advanced, and its factors."""
         counts = group.setdefault("device_step", {})
         key = str(device)
         if key not in counts:
@@ -238,7 +254,7 @@ class AdamW(torch.optim.Optimizer):
             counts[key] = (torch.zeros(1, dtype=torch.int64, device=device), torch.empty(3, dtype=torch.float32, device=device))
         count, factors = counts[key]
         adamw_tick(count, factors, lr=group["lr"], betas=group["betas"], weight_decay=group["weight_decay"])
-        return factors
+        return count, factors
 
     def state_dict(self):
         out = super().state_dict()

@@ -9,11 +9,21 @@
 // master weights (18 bytes each) take 125-134 us, 4.8-5.2 TB/s, and reading the moments out as float32 (10 bytes) 71.
 //
 // 8-bit moments.  256 consecutive values share an exponent E, that of the largest finite magnitude among them (at least
-// -126; stored plus 127).  A value is scaled by 2^-E -- exactly -- into [0, 2) and rounded to nearest even in a small
-// floating format: m has a sign, 4 exponent and 3 mantissa bits (0x80: not finite, read as NaN), v 5 and 3 (0xff: not
-// finite, read as infinity).  Half a step is 2^-4 of a value over 14 and 30 binades.  The update uses the fresh float32
-// m and v; only what the next step reads is rounded.  A v above 0 is never stored as 0: next step's division by
-// sqrt(v) would blow its m up.  (v loses accuracy only where it is 2^-30 of its block's largest.)
+// -126; stored plus 127).  A value is scaled by 2^-E -- exactly -- into [0, 2) and rounded in a small floating format: m has a
+// sign, 4 exponent and 3 mantissa bits (0x80: not finite, read as NaN), v 5 and 3 (0xff: not finite, read as infinity).  A step
+// of the codes is 2^-4 to 2^-3 of a value, over 14 and 30 binades.  The update uses the fresh float32 m and v; only what the
+// next step reads is rounded.  A v above 0 is never stored as 0: next step's division by sqrt(v) would blow its m up.
+//
+// How it is rounded.  One step changes v by some 1 - b2 of itself, a hundredth of a code step, and m by 1 - b1: rounded to
+// nearest, they stand still (a constant gradient leaves v at 0.014 of its value after 3000 steps and the parameters go five
+// times as far).  So a run of steps rounds up with the probability that the value has of the step above it: the moments are
+// then right on average, and noisy by a fifth of v at b2 = 0.999 (3000 steps of constant, random and shrinking gradients: mean
+// v 0.99 - 1.01 of the float32 one, parameters within 4 %).  The random bits are a hash of the step's number and the value's
+// index: runs repeat, and how tensors are grouped into calls changes nothing.  Nor may a magnitude be cut off at the largest
+// code's, 1.75 for v: a block whose largest is above that takes the next exponent.  The first kNearest steps round to nearest
+// all the same: the new gradient has a weight of 1 / 8 or more in them, so that moments do not stand still, and nearest is the
+// smaller error.  Callers of a single step (dither 0) get nearest, with magnitudes cut off at the largest code.  The hash and
+// the registers it holds cost 36 M bfloat16 values with masters 136 us instead of 121, 20 M 68 instead of 64.
 #include "cafe_dense.h"
 
 #include <algorithm>
@@ -31,6 +41,7 @@ constexpr int kItems = 48;              // tensors of one launch: their descript
 constexpr int lane_values(int bits) { return bits == 8 ? 8 : 4; }
 constexpr int span(int bits) { return 256 * lane_values(bits); }
 constexpr int kBlock = 256;
+constexpr int64_t kNearest = 8;         // first steps of a run, whose moments are rounded to nearest
 constexpr int64_t kGrid = 1 << 22;      // workgroups of a launch (a grid holds fewer than 2^32 work items); longer tensors go in pieces
 
 struct Item { void *p; const void *g; void *m, *v; uint8_t *me, *ve; float *w; int64_t n; };
@@ -40,6 +51,8 @@ struct AdamArgs {
     const float *factors;               // device: {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd}, or null
     float step_size, root, keep, b1, c1, b2, c2, eps;
     int count;
+    const int64_t *dither_dev;          // device: the number of the step, or null
+    int64_t dither, from;               // the number of the step; values of the first tensor that earlier launches took
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
@@ -102,13 +115,26 @@ template <bool SECOND> __device__ __forceinline__ float decode8(int c, int e) {
     if (SECOND) return c == 0xff ? INFINITY : v;
     return c == 0x80 ? NAN : c & 0x80 ? -v : v;
 }
-template <bool SECOND> __device__ __forceinline__ int encode8(float x, int e) {
+// 32 bits that look random, of a counter: two rounds of multiplying by an odd number and folding the high half back (the
+// numbers are fractions of the golden ratio and of the square roots of 2 and 3).
+constexpr uint32_t kGolden = 0x9E3779B9u;
+__device__ __forceinline__ uint32_t scramble(uint32_t h) {
+    h ^= h >> 16; h *= 0x6A09E667u;
+    h ^= h >> 15; h *= 0xBB67AE85u;
+    return h ^ (h >> 16);
+}
+__device__ __forceinline__ uint32_t dither_key(int64_t step, int64_t index) {
+    return scramble(scramble((uint32_t)step * kGolden + (uint32_t)(step >> 32)) + (uint32_t)(index >> 32));
+}
+// up: in [0, 1), what is added ahead of rounding down; negative: round to nearest even
+template <bool SECOND> __device__ __forceinline__ int encode8(float x, int e, float up) {
     constexpr int low = SECOND ? -30 : -14;
     const float mag = fabsf(x);
     if (!(mag <= 3.4028234663852886e38f)) return SECOND ? 0xff : 0x80;
     const float a = ldexpf(mag, -e);
     const int b = max(exponent_of(a), low);
-    int c = (int)rintf(ldexpf(a, 3 - b)) + 8 * (b - low);
+    const float steps = ldexpf(a, 3 - b);
+    int c = (int)(up < 0.f ? rintf(steps) : floorf(steps + up)) + 8 * (b - low);
     if (SECOND) {
         c = min(c, 0xfe);
         return c == 0 && mag > 0.f ? 1 : c;
@@ -116,21 +142,26 @@ template <bool SECOND> __device__ __forceinline__ int encode8(float x, int e) {
     c = min(c, 0x7f);
     return x < 0.f && c > 0 ? c | 0x80 : c;
 }
-// Exponents of a block of m and of v, eight values per lane of 32 lanes.  The largest magnitude's exponent is the largest
-// exponent, so both go through the lanes as the two halves of one word (0 .. 254; what is not finite counts as 0).
-__device__ __forceinline__ void block_exponents(const float *m, const float *v, int *em, int *ev) {
+// Exponents of a block of m and of v, eight values per lane of 32 lanes.  The largest magnitude has the largest exponent and
+// leading 7 mantissa bits, so both go through the lanes as the two halves of one word (what is not finite counts as 0).
+// ROOM: a block whose largest reaches the largest code takes the next exponent, so that it can be rounded up.
+template <bool ROOM> __device__ __forceinline__ void block_exponents(const float *m, const float *v, int *em, int *ev) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 top = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t a = (__float_as_uint(m[i]) >> 23) & 255, b = (__float_as_uint(v[i]) >> 23) & 255;
-        top = __builtin_elementwise_max(top, u16x2{(unsigned short)(a == 255 ? 0 : a), (unsigned short)(b == 255 ? 0 : b)});
+        const uint32_t a = (__float_as_uint(m[i]) >> 16) & 0x7fff, b = (__float_as_uint(v[i]) >> 16) & 0x7fff;
+        top = __builtin_elementwise_max(top, u16x2{(unsigned short)(a >= 0x7f80 ? 0 : a), (unsigned short)(b >= 0x7f80 ? 0 : b)});
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1)
         top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, __shfl_xor(__builtin_bit_cast(int, top), d, 64)));
-    *em = max((int)top.x - 127, -126);
-    *ev = max((int)top.y - 127, -126);
+    *em = max((top.x >> 7) - 127, -126);
+    *ev = max((top.y >> 7) - 127, -126);
+    if (ROOM) {                                         // 1.875 and 1.75 of that exponent; a byte holds no more than 127
+        *em = min(*em + ((top.x & 127) >= 0x70), 127);
+        *ev = min(*ev + ((top.y & 127) >= 0x60), 127);
+    }
 }
 
 __device__ __forceinline__ int item_of(const int32_t *first, int count, int block) {
@@ -144,7 +175,8 @@ __device__ __forceinline__ int item_of(const int32_t *first, int count, int bloc
 
 // PAST: a step over more than the caches hold.  Nothing of it is found there by the next step, so moments, masters and
 // gradients go past them and leave the room to the parameters, which the next forward reads.
-template <class T, bool BITS8, bool PAST> __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
+// DITHER: 8-bit moments of a run of steps.
+template <class T, bool BITS8, bool PAST, bool DITHER> __global__ __launch_bounds__(256) void k_adamw(AdamArgs a) {
     const int k = item_of(a.first, a.count, blockIdx.x);
     const Item t = a.t[k];
     float step_size = a.step_size, root = a.root, keep = a.keep;
@@ -180,9 +212,23 @@ template <class T, bool BITS8, bool PAST> __global__ __launch_bounds__(256) void
         for (int i = 0; i < L; i++)
             if (i >= n) m[i] = v[i] = 0.f;
         int em, ev, cm[L], cv[L];
-        block_exponents(m, v, &em, &ev);
+        int64_t run = 0;
+        if constexpr (DITHER) run = a.dither_dev ? *a.dither_dev : a.dither;
+        if (DITHER && run > kNearest) {
+            block_exponents<true>(m, v, &em, &ev);
+            const int64_t index = at + (k == 0 ? a.from : 0);
+            const uint32_t key = dither_key(run, index);
 #pragma unroll
-        for (int i = 0; i < L; i++) { cm[i] = encode8<false>(m[i], em); cv[i] = encode8<true>(v[i], ev); }
+            for (int i = 0; i < L; i++) {               // 20 bits each: steps below 16 and they add up exactly
+                const uint32_t h = scramble(((uint32_t)index + i) * kGolden + key);
+                cm[i] = encode8<false>(m[i], em, (float)((h << 16 | h >> 16) >> 12) * 0x1p-20f);
+                cv[i] = encode8<true>(v[i], ev, (float)(h >> 12) * 0x1p-20f);
+            }
+        } else {
+            block_exponents<false>(m, v, &em, &ev);
+#pragma unroll
+            for (int i = 0; i < L; i++) { cm[i] = encode8<false>(m[i], em, -1.f); cv[i] = encode8<true>(v[i], ev, -1.f); }
+        }
         put<L, PAST>((uint8_t *)t.m + at, n, cm);
         put<L, PAST>((uint8_t *)t.v + at, n, cv);
         if ((threadIdx.x & 31) == 0) { t.me[block] = (uint8_t)(em + 127); t.ve[block] = (uint8_t)(ev + 127); }
@@ -242,23 +288,35 @@ bool bad_hyper(const char *who, double lr, double b1, double b2, double eps, dou
 // take 115 and 95, 25 M bfloat16 ones (453 MB) 160 and 138.  Reading 38 M moments out twice (302 MB): 71 and 92 us.
 constexpr int64_t kPastStep = (int64_t)480 << 20, kPastValues = (int64_t)256 << 20;
 
-template <class T, bool BITS8> int launch(const AdamArgs &a, unsigned blocks, bool past, hipStream_t st) {
-    if (past) hipLaunchKernelGGL((k_adamw<T, BITS8, true>), dim3(blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_adamw<T, BITS8, false>), dim3(blocks), dim3(256), 0, st, a);
+template <class T, bool BITS8, bool DITHER> int launch(const AdamArgs &a, unsigned blocks, bool past, hipStream_t st) {
+    if (past) hipLaunchKernelGGL((k_adamw<T, BITS8, true, DITHER>), dim3(blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_adamw<T, BITS8, false, DITHER>), dim3(blocks), dim3(256), 0, st, a);
     CAFE_HIP_CHECK(hipGetLastError());
     return 0;
+}
+template <class T> int launch(const AdamArgs &a, unsigned blocks, bool past, bool eight, hipStream_t st) {
+    if (!eight) return launch<T, false, false>(a, blocks, past, st);
+    if (a.dither_dev || a.dither > kNearest) return launch<T, true, true>(a, blocks, past, st);
+    return launch<T, true, false>(a, blocks, past, st);
 }
 
 }  // namespace
 
 extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
                               double eps, double weight_decay, int64_t step, const float *d_factors, cafe_stream_t stream) {
+    return cafe_adamw_dither_dev(tensors, count, dtype, state_bits, lr, beta1, beta2, eps, weight_decay, step, d_factors, 0, nullptr, stream);
+}
+
+extern "C" int cafe_adamw_dither_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
+                                     double eps, double weight_decay, int64_t step, const float *d_factors, int64_t dither,
+                                     const int64_t *d_dither, cafe_stream_t stream) {
     if (count < 0 || (count && !tensors)) { set_error("cafe_adamw_dev: no tensor table"); return 1; }
     if (dtype < kF32 || dtype > kF16 || (state_bits != 8 && state_bits != 32)) {
         set_error("cafe_adamw_dev: type code %d, %d-bit states", dtype, state_bits);
         return 1;
     }
     if (bad_hyper("cafe_adamw_dev", lr, beta1, beta2, eps, weight_decay)) return 1;
+    if (dither < 0) { set_error("cafe_adamw_dev: dither %lld, 0 or the number of the step expected", (long long)dither); return 1; }
     if (!d_factors && step < 1) { set_error("cafe_adamw_dev: step %lld, the first is 1", (long long)step); return 1; }
     for (int i = 0; i < count; i++) {
         const int64_t *c = tensors + i;
@@ -273,6 +331,7 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
     }
     AdamArgs a = {};
     a.factors = d_factors;
+    a.dither = dither; a.dither_dev = d_dither;
     if (!d_factors) {
         a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
         a.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
@@ -295,6 +354,7 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
             auto on = [&](int f, int64_t bytes) { return at(f) ? (void *)(at(f) + bytes) : nullptr; };
             const int64_t left = tensors[7 * (int64_t)count + i] - from, n = std::min<int64_t>(left, (kGrid - blocks) * span(state_bits));
             if (left == 0) { i++; from = 0; continue; }
+            if (a.count == 0) a.from = from;
             const int64_t e = from * (dtype == kF32 ? 4 : 2), s = state_bits == 8 ? from : from * 4;
             a.t[a.count] = Item{on(0, e), on(1, e), on(2, s), on(3, s), (uint8_t *)on(4, from / kBlock), (uint8_t *)on(5, from / kBlock),
                                 (float *)on(6, from * 4), n};
@@ -306,10 +366,8 @@ extern "C" int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int 
         a.first[a.count] = (int32_t)blocks;
         const unsigned b = (unsigned)blocks;
         const bool s8 = state_bits == 8;
-        int rc;
-        if (dtype == kF32) rc = s8 ? launch<float, true>(a, b, past, st) : launch<float, false>(a, b, past, st);
-        else if (dtype == kBF16) rc = s8 ? launch<__bf16, true>(a, b, past, st) : launch<__bf16, false>(a, b, past, st);
-        else rc = s8 ? launch<_Float16, true>(a, b, past, st) : launch<_Float16, false>(a, b, past, st);
+        const int rc = dtype == kF32 ? launch<float>(a, b, past, s8, st) : dtype == kBF16 ? launch<__bf16>(a, b, past, s8, st)
+                                                                                       : launch<_Float16>(a, b, past, s8, st);
         if (rc) return rc;
     }
     return 0;

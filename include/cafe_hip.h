@@ -374,6 +374,14 @@ int cafe_interact_bwd_dev(const void *d_dout, int64_t lddo, const void *d_x, int
  * lr and step are not used, so that the call can be captured and replayed. */
 int cafe_adamw_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
                    double eps, double weight_decay, int64_t step, const float *d_factors, cafe_stream_t stream);
+/* The same for a step of a run (cafe_adamw_dev is the call with dither 0 and no d_dither).  8-bit moments are rounded to
+ * nearest in the first eight steps and where dither is 0; from the ninth step on up or down with the probabilities that
+ * leave their mean in place: rounded to nearest they would stand still, one step changes them by less than half a code.  The
+ * random bits are a hash of the step's number and the value's index in its tensor.  dither: that number; d_dither != null:
+ * read from the device.  No effect on 32-bit moments. */
+int cafe_adamw_dither_dev(const int64_t *tensors, int count, int dtype, int state_bits, double lr, double beta1, double beta2,
+                          double eps, double weight_decay, int64_t step, const float *d_factors, int64_t dither,
+                          const int64_t *d_dither, cafe_stream_t stream);
 /* *d_step += 1, then d_factors[3] for that step.  d_lr != null: the learning rate is read from there. */
 int cafe_adamw_tick_dev(int64_t *d_step, const float *d_lr, double lr, double beta1, double beta2, double weight_decay,
                         float *d_factors, cafe_stream_t stream);
