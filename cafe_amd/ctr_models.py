@@ -3,9 +3,9 @@
 The embedding layer is cafe_amd.CafeEmbeddingCollection, i.e. the fused HIP launches; the heads are stock torch ops by
 default (dense_ops="torch") or, with dense_ops="hip", the package's own launches over the same parameters: every layer
 with its bias and activation (and WDL's wide logit) through cafe_amd.linear, the interaction through cafe_amd.interact.
-dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; embedding rows and
-the loss stay float32; cafe_amd.adamw.AdamW keeps float32 master weights for such parameters).  Structure and
-initialisation follow the reference:
+dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; embedding rows stay
+float32, and train_step's loss is taken in float32 from the logit, not from the rounded probability;
+cafe_amd.adamw.AdamW keeps float32 master weights for such parameters).  Structure and initialisation follow the reference:
 
 * DLRM: bottom MLP -> dot interaction of [x] + embeddings, strictly-lower-triangle terms, concatenated behind x ->
   top MLP whose last layer is a sigmoid (dlrm_s_pytorch.py:213-251 create_mlp, :779-820 interact_features,
@@ -33,6 +33,7 @@ cafe_amd.adamw.AdamW steps them in one launch)."""
 import numpy as np
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import config as cfg
 from .collection import CafeEmbeddingCollection
@@ -73,6 +74,26 @@ def interact_dot(x, ly, itself=False):
     lj = torch.tensor([j for i in range(ni) for j in range(i + off)], device=Z.device)
     zflat = Z[:, li, lj]
     return zflat if x is None else torch.cat([x, zflat], dim=1)
+
+
+class _Probability(torch.autograd.Function):
+    """A rounded probability in float32, for a loss that divides by p (1 - p).  Its layer's backward multiplies by the slope of
+    the unrounded one, which cancels that division to within a factor of 1.5 (half a step of the rounding) wherever p is
+    neither 0 nor 1.  There it has nothing to cancel, and nothing passes, as through torch.sigmoid."""
+
+    @staticmethod
+    def forward(ctx, y):
+        ctx.save_for_backward(y)
+        return y.to(torch.float32, copy=True)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        y, = ctx.saved_tensors
+        g = g.masked_fill((y == 0) | (y == 1), 0.0)
+        if y.dtype is torch.float16:                              # 1 / p passes its range from 1.5e-5 down
+            g = g.clamp(-65504.0, 65504.0)
+        return g.to(y.dtype)
 
 
 class CafeCTRHead(nn.Module):
@@ -128,27 +149,39 @@ class CafeCTRHead(nn.Module):
         if dense_dtype != torch.float32:
             self.to(dense_dtype)
 
-    def _forward_hip(self, dense, emb):
-        """forward() over cafe_amd.linear and cafe_amd.interact; activations in dense_dtype, the result float32."""
+    def _forward_hip(self, dense, emb, logits):
+        """forward() or logits() over cafe_amd.linear and cafe_amd.interact; activations in dense_dtype, the result float32."""
         t = self.dense_dtype
         dense = dense.to(t) if self.dense_dim else None
         if self.kind == "dlrm":
             x = run_mlp(self.bot_l, dense) if self.dense_dim else None
-            return run_mlp(self.top_l, dot_interaction(x, emb, self.interaction_itself, dtype=t)).float()
+            z = dot_interaction(x, emb, self.interaction_itself, dtype=t)
+            return run_mlp(list(self.top_l)[:-1], z).float() if logits else _Probability.apply(run_mlp(self.top_l, z))
         z = emb.transpose(0, 1).reshape(emb.shape[1], -1).to(t)
         if self.dense_dim:
             z = torch.cat([dense, z], dim=1)
         if self.kind == "wdl":                                    # the wide logit enters the last deep layer's launch
-            return torch.sigmoid(run_mlp(self.top_l, z, residual=linear(z, self.wide.weight, self.wide.bias)).float())
+            z = run_mlp(self.top_l, z, residual=linear(z, self.wide.weight, self.wide.bias)).float()
+            return z if logits else torch.sigmoid(z)
         x1 = z
         for i in range(self.cross_layer_n):                       # x_l w is a layer of one output
             x1 = z * linear(x1, getattr(self, f"cross_weight_{i}").t()) + getattr(self, f"cross_bias_{i}")
-        return linear(torch.cat([run_mlp(self.top_l, z), x1], dim=1), self.last_layer.weight, self.last_layer.bias, "sigmoid").float()
+        z = torch.cat([run_mlp(self.top_l, z), x1], dim=1)
+        if logits:
+            return linear(z, self.last_layer.weight, self.last_layer.bias).float()
+        return _Probability.apply(linear(z, self.last_layer.weight, self.last_layer.bias, "sigmoid"))
+
+    def logits(self, dense, emb):
+        """emb: [F, B, D] -> the logit of the click probability, [B, 1] float32 (dense_ops="hip").  What a loss is taken from:
+        a probability next to 0 or 1 has lost its distance to them to rounding, and the loss divides by that distance."""
+        if self.dense_ops != "hip":
+            raise ValueError("logits() is dense_ops='hip''s; the torch head's loss is taken from its probability, as the reference's is")
+        return self._forward_hip(dense, emb, True)
 
     def forward(self, dense, emb):
         """emb: [F, B, D] -> click probability [B, 1]."""
         if self.dense_ops == "hip":
-            return self._forward_hip(dense, emb)
+            return self._forward_hip(dense, emb, False)
         B = emb.shape[1]
         if self.kind == "dlrm":
             x = self.bot_l(dense) if self.dense_dim else None
@@ -221,14 +254,28 @@ class CafeCTRModel(nn.Module):
         self.loss_fn = nn.BCELoss(reduction="mean")               # dlrm_s_pytorch.py:462, wdl.py:425, dcn.py:433
         self.to(dev)
 
-    def forward(self, dense, ids):
-        """dense: [B, dense_dim] or None; ids: [F, B] int64 local ids on the device."""
+    def _rows(self, ids):
         if not self.plain_idx:
-            return self.head(dense, _Lookup.apply(self._anchor, self, ids))
+            return _Lookup.apply(self._anchor, self, ids)
         sk = _Lookup.apply(self._anchor, self, ids[self.sk_idx].contiguous())
         pl = torch.stack([e(ids[i]) for e, i in zip(self.plain, self.plain_idx)])
-        emb = torch.cat([sk, pl]).index_select(0, self._order.to(sk.device))
-        return self.head(dense, emb)
+        return torch.cat([sk, pl]).index_select(0, self._order.to(sk.device))
+
+    def forward(self, dense, ids):
+        """dense: [B, dense_dim] or None; ids: [F, B] int64 local ids on the device."""
+        return self.head(dense, self._rows(ids))
+
+    def logits(self, dense, ids):
+        """CafeCTRHead.logits behind the embedding layer (dense_ops="hip")."""
+        return self.head.logits(dense, self._rows(ids))
+
+    def loss(self, dense, ids, labels):
+        """What train_step differentiates: loss_fn of the click probability.  dense_ops="hip" takes BCELoss's value from the
+        logit instead, where its gradient is p - label whatever the logit and the head's type."""
+        if self.head.dense_ops == "hip" and type(self.loss_fn) is nn.BCELoss:
+            return nn.functional.binary_cross_entropy_with_logits(self.logits(dense, ids), labels, self.loss_fn.weight,
+                                                                  reduction=self.loss_fn.reduction)
+        return self.loss_fn(self.forward(dense, ids), labels)
 
     def _lookup_out(self, ids, ahead):
         """Two output arrays used by alternate steps (ahead = 1: the one the NEXT forward will write), so that the next
@@ -254,8 +301,7 @@ class CafeCTRModel(nn.Module):
         fields sketch fields): that step's embedding forward is then queued behind this step's update before the host
         waits for the device's verdict on the insert (cafe_forward_hint_dev)."""
         optimizer.zero_grad(set_to_none=True)
-        p = self.forward(dense, ids)
-        loss = self.loss_fn(p, labels)
+        loss = self.loss(dense, ids, labels)
         loss.backward()
         if next_ids is not None and not self.plain_idx:
             self.embedding.hint_next(next_ids, self._lookup_out(next_ids, 1))

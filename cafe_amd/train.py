@@ -109,9 +109,14 @@ def evaluate(model, batches):
     tot, n, hit = 0.0, 0, 0
     with torch.no_grad():
         for x, ids, y in batches:
-            p = model(x, ids)
-            tot += float(torch.nn.functional.binary_cross_entropy(p, y, reduction="sum"))
-            hit += int(((p > 0.5).float() == y).sum())
+            if model.head.dense_ops == "hip":                       # as train_step: the loss of the logit
+                z = model.logits(x, ids)
+                tot += float(torch.nn.functional.binary_cross_entropy_with_logits(z, y, reduction="sum"))
+                hit += int(((z > 0).float() == y).sum())
+            else:
+                p = model(x, ids)
+                tot += float(torch.nn.functional.binary_cross_entropy(p, y, reduction="sum"))
+                hit += int(((p > 0.5).float() == y).sum())
             n += y.numel()
     return tot / max(n, 1), hit / max(n, 1)
 
