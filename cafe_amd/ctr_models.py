@@ -38,7 +38,7 @@ from torch.autograd.function import once_differentiable
 from . import config as cfg
 from .collection import CafeEmbeddingCollection
 from .interact import dot_interaction
-from .linear import DTYPE_CODE, linear, run_mlp
+from .linear import DTYPE_CODE, linear, mlp_modules, run_mlp
 
 
 def create_mlp(ln, sigmoid_layer=-1, rng=None):
@@ -156,7 +156,7 @@ class CafeCTRHead(nn.Module):
         if self.kind == "dlrm":
             x = run_mlp(self.bot_l, dense) if self.dense_dim else None
             z = dot_interaction(x, emb, self.interaction_itself, dtype=t)
-            return run_mlp(list(self.top_l)[:-1], z).float() if logits else _Probability.apply(run_mlp(self.top_l, z))
+            return run_mlp(mlp_modules(self.top_l)[:-1], z).float() if logits else _Probability.apply(run_mlp(self.top_l, z))
         z = emb.transpose(0, 1).reshape(emb.shape[1], -1).to(t)
         if self.dense_dim:
             z = torch.cat([dense, z], dim=1)

@@ -214,22 +214,44 @@ def linear_backward(grad, x, weight, kept=None, activation="none", need=(True, T
         return _backward(grad, x, weight, kept, act, tuple(need))
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _plain(module):
+    """Raises unless calling `module` is its class's forward and nothing else: run_mlp goes by what the class stands for."""
+    if any(getattr(module, h) for h in _HOOKS) or nn.modules.module._has_any_global_hook():
+        raise ValueError(f"{type(module).__name__} with hooks (weight_norm registers one): run_mlp would pass them by")
+    if "forward" in vars(module):
+        raise ValueError(f"{type(module).__name__} with a forward of its own: run_mlp would pass it by")
+    return module
+
+
 _ACTIVATION_OF = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}
+
+
+def mlp_modules(layers):
+    """The modules of an nn.Sequential or a list, as run_mlp takes them; refuses what it refuses of the container."""
+    if isinstance(layers, nn.Module):
+        if type(layers) is not nn.Sequential:
+            raise ValueError(f"nn.Sequential or a list of modules expected, not {type(layers).__name__}")
+        _plain(layers)
+    return [_plain(m) for m in layers]
 
 
 def run_mlp(layers, x, residual=None):
     """An nn.Sequential of nn.Linear layers, each followed by its activation module or by the next Linear, one launch per
-    layer; `residual` is added to the last layer's output."""
-    mods = list(layers)
+    layer; `residual` is added to the last layer's output.  `layers` may be a list of such modules.  What their classes do is
+    done, so modules whose call does something else are refused: subclasses (a parametrized Linear is one), hooks."""
+    mods = mlp_modules(layers)
     at = 0
     while at < len(mods):
         lin = mods[at]
-        if not isinstance(lin, nn.Linear):
-            raise ValueError(f"nn.Linear expected at {at}, not {type(lin).__name__}")
+        if type(lin) is not nn.Linear:
+            raise ValueError(f"nn.Linear itself expected at {at}, not {type(lin).__name__}")
         act, step = "none", 1
         if at + 1 < len(mods) and not isinstance(mods[at + 1], nn.Linear):
             nxt = mods[at + 1]
-            exact_gelu = isinstance(nxt, nn.GELU) and nxt.approximate == "none"
+            exact_gelu = type(nxt) is nn.GELU and nxt.approximate == "none"
             act = "gelu" if exact_gelu else _ACTIVATION_OF.get(type(nxt))
             if act is None:
                 raise ValueError(f"activation module {nxt} has no fused form")
