@@ -76,6 +76,9 @@ def interact_dot(x, ly, itself=False):
     return zflat if x is None else torch.cat([x, zflat], dim=1)
 
 
+_SIGMOID = nn.Sigmoid()
+
+
 class _Probability(torch.autograd.Function):
     """A rounded probability in float32, for a loss that divides by p (1 - p).  Its layer's backward multiplies by the slope of
     the unrounded one, which cancels that division to within a factor of 1.5 (half a step of the rounding) wherever p is
@@ -161,15 +164,13 @@ class CafeCTRHead(nn.Module):
         if self.dense_dim:
             z = torch.cat([dense, z], dim=1)
         if self.kind == "wdl":                                    # the wide logit enters the last deep layer's launch
-            z = run_mlp(self.top_l, z, residual=linear(z, self.wide.weight, self.wide.bias)).float()
+            z = run_mlp(self.top_l, z, residual=run_mlp([self.wide], z)).float()
             return z if logits else torch.sigmoid(z)
         x1 = z
         for i in range(self.cross_layer_n):                       # x_l w is a layer of one output
             x1 = z * linear(x1, getattr(self, f"cross_weight_{i}").t()) + getattr(self, f"cross_bias_{i}")
         z = torch.cat([run_mlp(self.top_l, z), x1], dim=1)
-        if logits:
-            return linear(z, self.last_layer.weight, self.last_layer.bias).float()
-        return _Probability.apply(linear(z, self.last_layer.weight, self.last_layer.bias, "sigmoid"))
+        return run_mlp([self.last_layer], z).float() if logits else _Probability.apply(run_mlp([self.last_layer, _SIGMOID], z))
 
     def logits(self, dense, emb):
         """emb: [F, B, D] -> the logit of the click probability, [B, 1] float32 (dense_ops="hip").  What a loss is taken from:

@@ -76,3 +76,22 @@ def test_allowed():
     for mods in (layers(), list(layers()), layers()[:-1], nn.Sequential(nn.Linear(5, 7), nn.GELU())):
         with pytest.raises(_lib.CafeError, match="GPU"):
             run_mlp(mods, X)
+
+
+def test_layers_beside_the_stacks():
+    """WDL's wide layer and DCN's last one are modules too."""
+    from cafe_amd.ctr_models import CafeCTRHead
+    head = CafeCTRHead("wdl", 4, 8, 13, dense_ops="hip")
+    hooked(head.wide, "register_forward_pre_hook")
+    with pytest.raises(ValueError, match="hooks"):
+        head(torch.rand(6, 13), torch.randn(4, 6, 8))
+
+
+@pytest.mark.gpu
+def test_last_layer_of_dcn():
+    from cafe_amd.ctr_models import CafeCTRHead
+    head = CafeCTRHead("dcn", 4, 8, 13, dense_ops="hip").cuda()
+    hooked(head.last_layer, "register_forward_hook")
+    for call in (head, head.logits):
+        with pytest.raises(ValueError, match="hooks"):
+            call(torch.rand(6, 13, device="cuda"), torch.randn(4, 6, 8, device="cuda"))
