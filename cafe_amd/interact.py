@@ -7,7 +7,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .linear import DTYPE_CODE, launch_on, on_device
+from .linear import DTYPE_CODE, differentiated, launch_on, on_device
 
 MAX_FEATURES = 128
 
@@ -77,6 +77,6 @@ def dot_interaction(x, emb, itself=False, dtype=None):
     if not 1 <= nf <= MAX_FEATURES:
         raise ValueError(f"{nf} feature rows: 1 .. {MAX_FEATURES} expected")
     on_device(emb)
-    if torch.is_grad_enabled() and (emb.requires_grad or (x is not None and x.requires_grad)):
+    if differentiated(x, emb):
         return _Interact.apply(x, emb, bool(itself), dtype)
     return _forward(x, emb, bool(itself), dtype)

@@ -13,6 +13,7 @@ from typing import NamedTuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -31,6 +32,12 @@ def on_device(t):
     """Raises unless `t` lives on a GPU (there is no CPU path)."""
     if not t.is_cuda:
         raise _lib.CafeError("cafe_amd needs GPU tensors: there is no CPU path in this package")
+
+
+def differentiated(*tensors):
+    """Whether a call on `tensors` (or None) goes through its autograd function: one requires grad, or a level of forward-mode
+    differentiation is open.  There one may carry a tangent, without requiring grad; the function raises for it."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or forward_ad._current_level >= 0
 
 
 class launch_on:
@@ -174,7 +181,7 @@ def linear(x, weight, bias=None, activation="none", residual=None):
         residual = residual.expand(*lead, n).reshape(-1, n) if x.dim() != 2 or residual.shape != (lead[0], n) else residual
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty(lead.numel(), 0)
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if differentiated(x, weight, bias, residual):
         y = _Linear.apply(x2, weight, bias, residual, act)
     else:
         y = _forward(x2, weight, bias, act, residual, False)[0]
