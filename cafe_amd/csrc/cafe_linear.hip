@@ -86,7 +86,7 @@ template <int ACT> __device__ __forceinline__ float through(float dy, float kept
     if (ACT == ACT_SLOPE) return kept == 0.f ? 0.f : dy * kept;
     float s;
     activate<ACT, true>(kept, &s);
-    return dy * s;
+    return s == 0.f ? 0.f : dy * s;
 }
 
 // Where a product's result goes.  part != null: float32 partial sums of one slice of the reduction, joined by k_join.
