@@ -89,6 +89,7 @@ SYMBOLS = {
     "cafe_linear_fwd_ws": (_i64, [_i64, _i64, _i64, ctypes.c_int]),
     "cafe_linear_fwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
                                            ctypes.c_int, ctypes.c_int, _vp, _i64, _vp]),
+    "cafe_linear_plan": (ctypes.c_int, [_i64, _i64, _i64] + [ctypes.c_int] * 3 + [_i32p]),
     "cafe_linear_bwd_ws": (_i64, [_i64, _i64, _i64, ctypes.c_int, ctypes.c_int]),
     "cafe_linear_bwd_dev": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
                                            ctypes.c_int, ctypes.c_int, _vp, _i64, _vp]),

@@ -992,6 +992,16 @@ extern "C" int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype
     return bwd_ws(m, k, n, dtype, act).bytes;
 }
 
+extern "C" int cafe_linear_plan(int64_t m, int64_t k, int64_t n, int dtype, int act, int product, int *tile) {
+    if (bad_sizes("cafe_linear_plan", m, k, n, dtype, act, ACT_SLOPE + 1)) return 1;
+    if (product < 0 || product > 2 || !tile) { set_error("cafe_linear_plan: product %d, or no array", product); return 1; }
+    const int parts = product ? dz_parts(dtype, act) : 1;
+    const Plan p = product == 0 ? plan(m, n, k, dtype) : product == 1 ? plan(m, k, n, dtype, parts) : plan(n, k, m, dtype, parts);
+    const bool few = product == 0 && is_skinny(m, k, n, dtype, true);
+    tile[0] = few ? 0 : p.bm; tile[1] = few ? 0 : p.bn; tile[2] = few ? 1 : p.slices; tile[3] = parts;
+    return 0;
+}
+
 extern "C" int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, const void *d_res,
                                    int64_t ldr, void *d_y, int64_t ldy, float *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
                                    int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream) {

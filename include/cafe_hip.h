@@ -338,6 +338,10 @@ int64_t cafe_linear_fwd_ws(int64_t m, int64_t k, int64_t n, int dtype);
 int cafe_linear_fwd_dev(const void *d_x, int64_t ldx, const void *d_w, int64_t ldw, const void *d_bias, const void *d_res,
                         int64_t ldr, void *d_y, int64_t ldy, float *d_kept, int64_t ldk, int64_t m, int64_t k, int64_t n,
                         int dtype, int act, void *d_ws, int64_t ws_bytes, cafe_stream_t stream);
+/* How a layer's product is cut up (product: 0 forward, 1 dx, 2 dw; act as in the backward): tile[4] = rows and columns of a
+ * tile (0, 0: the forward for few rows or outputs, of rows on boundaries of 4 bytes), slices of the reduction, parts of dz (2:
+ * half a tile's rows are the second part's).  For tests and timings; nothing is launched. */
+int cafe_linear_plan(int64_t m, int64_t k, int64_t n, int dtype, int act, int product, int *tile);
 /* Gradients of the same: dz = dy * act'(kept); dx[M, K] = dz w, dw[N, K] = dz^T x (contiguous), db[N] = column sums of dz.
  * Any of d_dx, d_dw, d_db may be null (not wanted).  d_kept [M, N]: for act 2, 3, 4 the value before the activation; for
  * relu that or its output (only the sign is read), of type `dtype`; for act 5 the float32 slopes act'(z) of any
