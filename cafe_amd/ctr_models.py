@@ -3,8 +3,8 @@
 The embedding layer is cafe_amd.CafeEmbeddingCollection, i.e. the fused HIP launches; the heads are stock torch ops by
 default (dense_ops="torch") or, with dense_ops="hip", the package's own launches over the same parameters: every layer
 with its bias and activation (and WDL's wide logit) through cafe_amd.linear, the interaction through cafe_amd.interact.
-dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; embedding rows stay
-float32, and train_step's loss is taken in float32 from the logit, not from the rounded probability;
+dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; float16 for inference,
+train_step refuses it: the gradients of a mean over a batch are below its range; embedding rows stay float32, and train_step's loss is taken in float32 from the logit, not from the rounded probability;
 cafe_amd.adamw.AdamW keeps float32 master weights for such parameters).  Structure and initialisation follow the reference:
 
 * DLRM: bottom MLP -> dot interaction of [x] + embeddings, strictly-lower-triangle terms, concatenated behind x ->
@@ -77,6 +77,8 @@ def interact_dot(x, ly, itself=False):
 
 
 _SIGMOID = nn.Sigmoid()
+NO_F16_TRAINING = ("a float16 head is for inference: the mean loss's gradients, 1 / batch and below, are under float16's normal range "
+                   "(6.1e-5) and would lose their digits or become 0; train in float32 or bfloat16")
 
 
 class _Probability(torch.autograd.Function):
@@ -301,6 +303,8 @@ class CafeCTRModel(nn.Module):
         next_ids: the next step's ids when the data loader has them already (contiguous [F, B] int64 on the device, all
         fields sketch fields): that step's embedding forward is then queued behind this step's update before the host
         waits for the device's verdict on the insert (cafe_forward_hint_dev)."""
+        if self.head.dense_dtype == torch.float16:
+            raise ValueError(NO_F16_TRAINING)
         optimizer.zero_grad(set_to_none=True)
         loss = self.loss(dense, ids, labels)
         loss.backward()

@@ -18,7 +18,7 @@ import torch
 
 from . import config as cfg
 from .adamw import AdamW
-from .ctr_models import CafeCTRModel
+from .ctr_models import NO_F16_TRAINING, CafeCTRModel
 from .data import BinaryCTRDataset
 
 
@@ -38,10 +38,11 @@ def parse(argv=None):
     p.add_argument("--learning-rate", type=float, default=0.1)
     p.add_argument("--dense-ops", choices=("torch", "hip"), default="torch",
                    help="the head's layers and interaction: stock torch ops, or the package's own launches")
-    p.add_argument("--dense-dtype", choices=("f32", "bf16", "f16"), default="f32", help="the head's type (bf16 / f16: --dense-ops hip)")
+    p.add_argument("--dense-dtype", choices=("f32", "bf16", "f16"), default="f32",
+                   help="the head's type (bf16: --dense-ops hip and an optimizer with master weights; f16 is not trained)")
     p.add_argument("--optimizer", choices=("sgd", "adamw", "adamw8bit"), default="sgd",
                    help="of the dense parameters (adamw: cafe_amd.adamw); the embedding tables keep their fused SGD")
-    p.add_argument("--dense-learning-rate", type=float, default=None, help="of the dense parameters (default: --learning-rate)")
+    p.add_argument("--dense-learning-rate", type=float, default=None, help="of the dense parameters (default: --learning-rate with sgd, 0.001 with adamw)")
     p.add_argument("--weight-decay", type=float, default=0.01, help="of adamw")
     p.add_argument("--num-batches", type=int, default=100)
     p.add_argument("--nepochs", type=int, default=1)
@@ -55,7 +56,15 @@ def parse(argv=None):
     p.add_argument("--num-fields", type=int, default=26)
     p.add_argument("--save-model", default="")
     p.add_argument("--load-model", default="")
-    return p.parse_args(argv)
+    a = p.parse_args(argv)
+    if a.dense_dtype == "f16":
+        p.error("--dense-dtype f16: " + NO_F16_TRAINING)
+    if a.dense_dtype == "bf16" and a.optimizer == "sgd":
+        p.error("--dense-dtype bf16 needs --optimizer adamw or adamw8bit, which keep float32 master weights: sgd adds its steps to "
+                "parameters of 8 bits, where most of them are lost to rounding")
+    if a.dense_learning_rate is None:
+        a.dense_learning_rate = a.learning_rate if a.optimizer == "sgd" else 1e-3
+    return a
 
 
 def synthetic_batches(w, dense_dim, num_batches, seed, device, start=0):
@@ -148,8 +157,7 @@ def main(argv=None):
                          adjust_thres=a.adjust_threshold, alpha=a.sketch_alpha, ln_bot=ln_bot, ln_top=ln_top, device=dev,
                          seed=a.numpy_rand_seed, per_field_calls=not a.fused_insert, dense_ops=a.dense_ops,
                          dense_dtype={"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[a.dense_dtype])
-    opt = make_optimizer(a.optimizer, model.dense_parameters(),
-                         a.learning_rate if a.dense_learning_rate is None else a.dense_learning_rate, a.weight_decay)
+    opt = make_optimizer(a.optimizer, model.dense_parameters(), a.dense_learning_rate, a.weight_decay)
     step0 = load_checkpoint(a.load_model, model, opt) if a.load_model else 0
     print(json.dumps({"model": a.model, "fields": len(counts), "dim": dim, "batch": batch, "hotn": model.hotn,
                       "cold_rows": int(sum(model.hash_sizes)), "ids": int(sum(counts)), "start_step": step0}), flush=True)
