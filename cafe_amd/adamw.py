@@ -176,7 +176,8 @@ class AdamW(torch.optim.Optimizer):
     parameters keep a float32 copy that the steps accumulate in (default True; ignored for float32).  capturable: the
     step count of a parameter group lives on the device, so that step() can be captured into a graph and replayed; lr may
     then be a float32 tensor of one element on the device, and parameters without a gradient are skipped but do not lag
-    behind the group's count.  Parameters are contiguous; sparse gradients are refused."""
+    behind the group's count.  Parameters are contiguous; sparse gradients are refused.  Master weights are what is stepped:
+    whoever writes 16-bit parameters in between (a checkpoint) clears `state` or loads the state that belongs to them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, master_weights=True,
                  capturable=False):
@@ -265,7 +266,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's, except that moments, codes and master weights keep their own types (torch casts floating state to the
-        parameter's)."""
+        parameter's).  Another optimizer's state is refused."""
+        for g in state_dict["param_groups"]:
+            if not self.defaults.keys() <= g.keys():
+                raise ValueError(f"not a state of this optimizer: no {sorted(self.defaults.keys() - g.keys())}")
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
