@@ -99,6 +99,20 @@ def save_checkpoint(path, model, step, optimizer=None):
                 **({"optimizer": state} if state["state"] else {})}, path)
 
 
+def restore_optimizer(optimizer, state):
+    """`state`: what a checkpoint holds for its optimizer, None if that had no state.  Then this one starts afresh: its moments
+    and master weights would be those of other parameters."""
+    if state is None:
+        optimizer.state.clear()
+        for g in optimizer.param_groups:
+            g.pop("device_step", None)
+        return
+    kind = lambda groups: [(set(g) - {"params", "device_step"}, len(g["params"]), g.get("state_bits")) for g in groups]    # noqa: E731
+    if kind(state["param_groups"]) != kind(optimizer.state_dict()["param_groups"]):
+        raise ValueError(f"the checkpoint's optimizer is another one than this {type(optimizer).__name__}, or over other parameters")
+    optimizer.load_state_dict(state)
+
+
 def load_checkpoint(path, model, optimizer=None):
     ck = torch.load(path, map_location="cpu", weights_only=True)
     emb = model.embedding
@@ -109,8 +123,8 @@ def load_checkpoint(path, model, optimizer=None):
     for w, src in zip(emb.weight_hash, ck["weight_hash"]):
         w.copy_(src)
     emb.sketch.load_state_tensors(ck["sketch"])
-    if optimizer is not None and "optimizer" in ck:
-        optimizer.load_state_dict(ck["optimizer"])
+    if optimizer is not None:
+        restore_optimizer(optimizer, ck.get("optimizer"))
     return int(ck["step"])
 
 
