@@ -173,6 +173,8 @@ def main(argv=None):
                          dense_dtype={"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[a.dense_dtype])
     opt = make_optimizer(a.optimizer, model.dense_parameters(), a.dense_learning_rate, a.weight_decay)
     step0 = load_checkpoint(a.load_model, model, opt) if a.load_model else 0
+    for g in opt.param_groups:                  # the command line's, as with sgd, whose checkpoints hold none
+        g["lr"], g["weight_decay"] = a.dense_learning_rate, a.weight_decay if "betas" in g else 0
     print(json.dumps({"model": a.model, "fields": len(counts), "dim": dim, "batch": batch, "hotn": model.hotn,
                       "cold_rows": int(sum(model.hash_sizes)), "ids": int(sum(counts)), "start_step": step0}), flush=True)
     step, run_loss, run_n, t0 = step0, None, 0, time.time()

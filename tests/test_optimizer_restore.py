@@ -45,3 +45,23 @@ def test_none():
         opt = stepped(name)
         train.restore_optimizer(opt, None)
         assert not opt.state
+
+
+@pytest.mark.gpu
+def test_a_resumed_run_steps_as_the_command_line_says(tmp_path):
+    common = ["--model", "wdl", "--workload", "cfg5", "--mini-batch-size", "128", "--dense-ops", "hip", "--optimizer", "adamw"]
+    path = str(tmp_path / "ck.pt")
+    train.main(common + ["--num-batches", "2", "--dense-learning-rate", "0.01", "--save-model", path])
+    seen = []
+    make = train.make_optimizer
+
+    def spy(*args):
+        seen.append(make(*args))
+        return seen[-1]
+    train.make_optimizer = spy
+    try:
+        train.main(common + ["--num-batches", "3", "--dense-learning-rate", "0.002", "--weight-decay", "0.03", "--load-model", path])
+    finally:
+        train.make_optimizer = make
+    g, = seen[0].param_groups
+    assert (g["lr"], g["weight_decay"]) == (0.002, 0.03) and {s["step"] for s in seen[0].state.values()} == {3}
