@@ -895,6 +895,11 @@ bool bad_sizes(const char *who, int64_t m, int64_t k, int64_t n, int dtype, int 
         set_error("%s: sizes %lld x %lld x %lld outside 0 .. 2^31 - 1", who, (long long)m, (long long)k, (long long)n);
         return true;
     }
+    const int64_t area = (int64_t)1 << 48;                  // values of a matrix: their bytes, twice and in slices, fit 63 bits
+    if (m * n > area || m * k > area || n * k > area) {
+        set_error("%s: a matrix of %lld x %lld x %lld has more than 2^48 values", who, (long long)m, (long long)k, (long long)n);
+        return true;
+    }
     if (dtype < kF32 || dtype > kF16) { set_error("%s: unknown type code %d", who, dtype); return true; }
     if (act < 0 || act >= acts) { set_error("%s: unknown activation code %d", who, act); return true; }
     return false;
