@@ -1,5 +1,5 @@
 // cafe_dense.h -- what the dense-side kernels (cafe_linear.hip, cafe_interact.hip, cafe_adamw.hip) share: element
-// types, 16-byte accesses at any element alignment, wave-wide sums.
+// types, 16-byte accesses at any element alignment, the 16 x 16 product, the order of tiles over the XCDs.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -95,6 +95,5 @@ __device__ __forceinline__ int xcd_tile(int id, int n) {
 }
 
 constexpr int kF32 = 0, kBF16 = 1, kF16 = 2;
-inline const char *dtype_name(int d) { return d == kF32 ? "float32" : d == kBF16 ? "bfloat16" : d == kF16 ? "float16" : "?"; }
 
 }  // namespace cafe

@@ -221,16 +221,16 @@ def linear_backward(grad, x, weight, kept=None, activation="none", need=(True, T
         return _backward(grad, x, weight, kept, act, tuple(need))
 
 
-_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
-
-
-def _plain(module):
-    """Raises unless calling `module` is its class's forward and nothing else: run_mlp goes by what the class stands for."""
-    if any(getattr(module, h) for h in _HOOKS) or nn.modules.module._has_any_global_hook():
-        raise ValueError(f"{type(module).__name__} with hooks (weight_norm registers one): run_mlp would pass them by")
-    if "forward" in vars(module):
-        raise ValueError(f"{type(module).__name__} with a forward of its own: run_mlp would pass it by")
-    return module
+def _plain(modules):
+    """Raises unless calling each is its class's forward and nothing else: run_mlp goes by what the class stands for."""
+    anywhere = nn.modules.module._has_any_global_hook()
+    for m in modules:
+        own = m.__dict__
+        if anywhere or own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"]:
+            raise ValueError(f"{type(m).__name__} with hooks (weight_norm registers one): run_mlp would pass them by")
+        if "forward" in own:
+            raise ValueError(f"{type(m).__name__} with a forward of its own: run_mlp would pass it by")
+    return modules
 
 
 _ACTIVATION_OF = {nn.ReLU: "relu", nn.Sigmoid: "sigmoid", nn.SiLU: "silu", nn.Identity: "none"}
@@ -241,8 +241,9 @@ def mlp_modules(layers):
     if isinstance(layers, nn.Module):
         if type(layers) is not nn.Sequential:
             raise ValueError(f"nn.Sequential or a list of modules expected, not {type(layers).__name__}")
-        _plain(layers)
-    return [_plain(m) for m in layers]
+        _plain([layers])
+        return _plain(list(layers._modules.values()))
+    return _plain(list(layers))
 
 
 def run_mlp(layers, x, residual=None):
