@@ -65,7 +65,7 @@ def dot_interaction(x, emb, itself=False, dtype=None):
     x: [B, D] (the bottom MLP's output) or None; emb: [F, B, D].  The result is [B, (D +) pairs] of `dtype` (default: x's
     type, emb's without x).  x has the result's type; emb has it too or is float32.  At most 128 feature rows, x included.
     Products and sums are float32.  Rows may be strided views.  Runs on the current stream of emb's device;
-    differentiable once in x and emb."""
+    differentiable once in x and emb, not in forward mode."""
     if emb.dim() != 3:
         raise ValueError(f"emb [fields, batch, dim] expected, not {tuple(emb.shape)}")
     dtype = (emb.dtype if x is None else x.dtype) if dtype is None else dtype

@@ -172,7 +172,7 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     x: [..., K] and weight: [N, K] (an nn.Linear's), bias: [N] or None, residual: anything that broadcasts to [..., N];
     all float32, bfloat16 or float16, on one GPU.  activation: "none", "relu", "sigmoid", "gelu" (z Phi(z)) or "silu".
     Rows may be strided views.  Runs on the current stream of x's device.  Differentiable once in x, weight, bias and
-    residual; the backward keeps x, weight and, for every activation but relu without a residual, one more [..., N]
+    residual, not in forward mode; the backward keeps x, weight and, for every activation but relu without a residual, one more [..., N]
     tensor, the activation's slopes in float32."""
     _check(x, weight, bias, activation, residual)
     lead = x.shape[:-1]
@@ -225,6 +225,8 @@ def _plain(modules):
     """Raises unless calling each is its class's forward and nothing else: run_mlp goes by what the class stands for."""
     anywhere = nn.modules.module._has_any_global_hook()
     for m in modules:
+        if not isinstance(m, nn.Module):
+            raise ValueError(f"modules expected, not {type(m).__name__}")
         own = m.__dict__
         if anywhere or own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"]:
             raise ValueError(f"{type(m).__name__} with hooks (weight_norm registers one): run_mlp would pass them by")

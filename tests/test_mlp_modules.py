@@ -52,6 +52,8 @@ CASES = {
     "pre-hook": lambda: nn.Sequential(hooked(nn.Linear(5, 7), "register_forward_pre_hook")),
     "backward hook": lambda: nn.Sequential(hooked(nn.Linear(5, 7), "register_full_backward_hook")),
     "hook of an activation": lambda: nn.Sequential(nn.Linear(5, 7), hooked(nn.ReLU(), "register_forward_hook")),
+    "a function": lambda: [nn.Linear(5, 7), torch.relu],
+    "a gap": lambda: [nn.Linear(5, 7), None],
     "hook of the Sequential": lambda: hooked(layers(), "register_forward_hook"),
 }
 
