@@ -5,9 +5,12 @@ Tolerance, per element: what two parts of a value leave of it is half a step of 
 normal range half the smallest subnormal, `tiny`), the slope's product half a float32 step; a float32 sum of n products is
 off by (n + 8) 2^-24 of their magnitudes twice over, and here every product comes in two parts, so (4 n + 16) 2^-24; then the
 result's own half step.  With one part the first term is u, which is more than the whole of the rest."""
+import ctypes
+
 import pytest
 import torch
 
+from cafe_amd import _lib
 from cafe_amd.linear import Slope, linear_backward
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +58,32 @@ def test_as_close_as_the_rounded_exact_gradients(t):
     dx, dw, dz, xd, wd = rounded_once(4096, 367, 256, t, seed=7)
     for got, want in ((dx, dz @ wd), (dw, dz.t() @ xd)):
         assert (got.double() - want).norm() <= 1.02 * (want.to(t).double() - want).norm()
+
+
+def test_parts_behind_32_bits():
+    """More than 2^32 values of dz: the second part starts behind them, and the last rows are theirs."""
+    t, m, k, n = torch.bfloat16, (1 << 20) + 3, 8, 4104
+    g = torch.Generator(device="cuda").manual_seed(1)
+    dy = torch.empty(m, n, dtype=t, device="cuda")
+    slopes = torch.empty(m, n, device="cuda")
+    for at in range(0, m, 1 << 17):
+        rows = min(1 << 17, m - at)
+        dy[at:at + rows] = torch.randn(rows, n, device="cuda", generator=g)
+        slopes[at:at + rows] = torch.rand(rows, n, device="cuda", generator=g) + 0.5
+    x, w = (torch.randn(s, k, device="cuda", generator=g).to(t) for s in (m, n))
+    dx, dw, db = linear_backward(dy, x, w, Slope(slopes), "silu")
+    u, tiny = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    for at in (0, m // 2, m - 300):
+        dz = dy[at:at + 300].double() * slopes[at:at + 300].double()
+        want, mag = dz @ w.double(), dz.abs() @ w.double().abs()
+        check(dx[at:at + 300], want, (u * u * 1.02 + (4 * n + 17) * U32) * mag + 1.01 * u * want.abs() + tiny, "dx")
+    out = (ctypes.c_int * 4)()
+    _lib.check(_lib.load().cafe_linear_plan(m, k, n, 1, 4, 2, out), "cafe_linear_plan")
+    row = -(-m // out[2]) + out[2]                              # additions in a row: a slice's and the slices'; db's, fewer than 2^12
+    for c in (0, n // 2, n - 1):
+        dz = dy[:, c].double() * slopes[:, c].double()
+        want, mag = dz @ x.double(), dz.abs() @ x.double().abs()
+        check(dw[c], want, (u * u * 1.02 + (4 * row + 17) * U32) * mag + 1.01 * u * want.abs() + tiny, "dw")
+        check(db[c:c + 1], dz.sum()[None], 2 ** 12 * U32 * dz.abs().sum()[None] + 1.01 * u * dz.sum().abs()[None], "db")
+    del dy, slopes, x, dx
+    torch.cuda.empty_cache()
