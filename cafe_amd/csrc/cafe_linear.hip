@@ -310,8 +310,9 @@ template <int MF, int R, int W, int V> __device__ __forceinline__ void weave() {
 // Bound by the matrix units where the reduction is long: 8192 x 4096 x 2048 takes 980 us in float32 (140 TF; library 912) and
 // 155-170 in bfloat16 with normally distributed operands (library 97-113; with uniform ones 132-143 and 87-90: the card's
 // clock follows what they toggle), 8192 x 1024 x 1024 139-145 and 22.5.  There the units are busy 76 % of a float32 launch
-// (counters), the rest is filling and storing.  Short reductions are bound by what surrounds the products, filling the pipeline and passing the tile through LDS: dx at
-// 16384 x 3341 with a reduction of 256 takes 70 us in bfloat16, 1.6 TB/s of stores (66 with rows on 16-byte boundaries).
+// (counters), the rest is filling and storing.  Short reductions are bound by what surrounds the products, filling the pipeline
+// and passing the tile through LDS: dx at 16384 x 3341 with a reduction of 256 takes 70 us in bfloat16, 1.6 TB/s of stores (66
+// with rows on 16-byte boundaries).
 //
 // PARTS 2: A is the sum of two matrices (dz's rounded values and what their rounding left).  The tile's BM entries are
 // BM / 2 rows of both, so that both meet the same B in LDS, and their products are added on the way out.  16384 x 3341 x 256

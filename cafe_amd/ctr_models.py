@@ -4,8 +4,9 @@ The embedding layer is cafe_amd.CafeEmbeddingCollection, i.e. the fused HIP laun
 default (dense_ops="torch") or, with dense_ops="hip", the package's own launches over the same parameters: every layer
 with its bias and activation (and WDL's wide logit) through cafe_amd.linear, the interaction through cafe_amd.interact.
 dense_dtype puts the head's parameters and activations in bfloat16 or float16 (dense_ops="hip" only; float16 for inference,
-train_step refuses it: the gradients of a mean over a batch are below its range; embedding rows stay float32, and train_step's loss is taken in float32 from the logit, not from the rounded probability;
-cafe_amd.adamw.AdamW keeps float32 master weights for such parameters).  Structure and initialisation follow the reference:
+train_step refuses it: the gradients of a mean over a batch are below its range; embedding rows stay float32, and
+train_step's loss is taken in float32 from the logit, not from the rounded probability; cafe_amd.adamw.AdamW keeps float32
+master weights for such parameters).  Structure and initialisation follow the reference:
 
 * DLRM: bottom MLP -> dot interaction of [x] + embeddings, strictly-lower-triangle terms, concatenated behind x ->
   top MLP whose last layer is a sigmoid (dlrm_s_pytorch.py:213-251 create_mlp, :779-820 interact_features,

@@ -115,6 +115,8 @@ def restore_optimizer(optimizer, state):
 
 def load_checkpoint(path, model, optimizer=None):
     ck = torch.load(path, map_location="cpu", weights_only=True)
+    if optimizer is not None:                   # first: what it refuses leaves the model as it was
+        restore_optimizer(optimizer, ck.get("optimizer"))
     emb = model.embedding
     model.head.load_state_dict(ck["head"])
     if "plain" in ck:
@@ -123,8 +125,6 @@ def load_checkpoint(path, model, optimizer=None):
     for w, src in zip(emb.weight_hash, ck["weight_hash"]):
         w.copy_(src)
     emb.sketch.load_state_tensors(ck["sketch"])
-    if optimizer is not None:
-        restore_optimizer(optimizer, ck.get("optimizer"))
     return int(ck["step"])
 
 

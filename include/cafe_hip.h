@@ -345,10 +345,9 @@ int cafe_linear_plan(int64_t m, int64_t k, int64_t n, int dtype, int act, int pr
 /* Gradients of the same: dz = dy * act'(kept); dx[M, K] = dz w, dw[N, K] = dz^T x (contiguous), db[N] = column sums of dz.
  * Any of d_dx, d_dw, d_db may be null (not wanted).  d_kept [M, N]: for act 2, 3, 4 the value before the activation; for
  * relu that or its output (only the sign is read), of type `dtype`; for act 5 the float32 slopes act'(z) of any
- * activation, as the forward wrote them; not read for act 0.  dz enters the products (they
- * run on the matrix units) as it is in float32 and where it needs no rounding (act 0, 1), else as two rounded parts, the
- * second what the rounding of the first left; db sums the unrounded values.  The
- * result does not depend on the run: every sum has a fixed order.
+ * activation, as the forward wrote them; not read for act 0.  dz enters the products (they run on the matrix units) as it
+ * is in float32 and where it needs no rounding (act 0, 1), else as two rounded parts, the second what the rounding of the
+ * first left; db sums the unrounded values.  The result does not depend on the run: every sum has a fixed order.
  * Workspace: cafe_linear_bwd_ws bytes (-1: bad sizes), on a boundary of 16 bytes. */
 int64_t cafe_linear_bwd_ws(int64_t m, int64_t k, int64_t n, int dtype, int act);
 int cafe_linear_bwd_dev(const void *d_dy, int64_t lddy, const void *d_x, int64_t ldx, const void *d_w, int64_t ldw,
